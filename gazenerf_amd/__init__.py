@@ -6,6 +6,8 @@ Public surface:
     PackedWeightCache
     merge_featmaps                                         (gazenerf_amd.merge)
     neural_render, NeuralRendererAMD                       (gazenerf_amd.upsample)
+    quantize_rows, int8_linear, write_featmaps,            (gazenerf_amd.int8; inference in 8 bits: a cache of feature maps and
+    read_featmaps, FeatureMapCache, QuantizedRows           the linear layers / 1x1 convolutions that read it)
     HotPathRenderer, MLPParams, GazeNeRFNetAMD             (gazenerf_amd.module; the last one is the whole
                                                            reference network: hot path -> merge -> upsampler x4)
     losses                                                 image losses + per-sample fitting step (SURVEY 8(f) N4,
@@ -22,5 +24,6 @@ Public surface:
 from . import data, gan, losses, perceptual, synth  # noqa: F401
 from .render import PackedWeightCache, importance_resample, render_two_stream, render_two_stream_tiled, sample_zvals  # noqa: F401
 from .merge import merge_featmaps  # noqa: F401
+from .int8 import FeatureMapCache, QuantizedRows, int8_linear, quantize_rows, read_featmaps, write_featmaps  # noqa: F401
 from .upsample import NeuralRendererAMD, neural_render  # noqa: F401
 from .module import GazeNeRFNetAMD, HotPathRenderer, MLPParams  # noqa: F401

@@ -16,6 +16,7 @@ WS_FWD, WS_FWD_SAVE, WS_BWD = 0, 1, 2
 STAGE_FWD_MLP, STAGE_DGRAD, STAGE_COMP_BWD, STAGE_WGRAD = 0, 1, 2, 3
 N_STAGES = 4
 ABI_VERSION = 4
+INT8_MAX_K = 131071
 
 _p = C.c_void_p
 
@@ -81,6 +82,21 @@ class GnrUpsampleWeights(C.Structure):
 GnrUpsampleWeightGrads = GnrUpsampleWeights      # identical layout (include/gnr.h)
 
 
+class GnrRowsProblem(_Sized):
+    _fields_ = [("struct_size", C.c_uint32), ("dtype", C.c_int32), ("channels_first", C.c_int32), ("batch", C.c_int32),
+                ("n_pix", C.c_int64), ("channels", C.c_int32), ("reserved", C.c_int32),
+                ("x", _p), ("x_batch", C.c_int64), ("x_stride", C.c_int64), ("q", _p), ("q_batch", C.c_int64), ("q_pitch", C.c_int64),
+                ("scale", _p), ("scale_batch", C.c_int64), ("slots", _p), ("n_slots", C.c_int64)]
+
+
+class GnrInt8Problem(_Sized):
+    _fields_ = [("struct_size", C.c_uint32), ("x_type", C.c_int32), ("y_type", C.c_int32), ("leaky", C.c_int32),
+                ("x_channels_first", C.c_int32), ("y_channels_first", C.c_int32), ("batch", C.c_int32), ("k", C.c_int32), ("o", C.c_int32),
+                ("reserved", C.c_int32), ("n_pix", C.c_int64), ("x", _p), ("x_batch", C.c_int64), ("x_stride", C.c_int64),
+                ("x_scale", _p), ("x_scale_batch", C.c_int64), ("slots", _p), ("n_slots", C.c_int64), ("w", _p), ("w_pitch", C.c_int64),
+                ("w_scale", _p), ("bias", _p), ("y", _p)]
+
+
 class GnrInputGrads(C.Structure):
     _fields_ = [("R", _p), ("T", _p), ("shape_code", _p), ("gaze", _p), ("appea_code", _p), ("ray_bias", _p * 2)]
 
@@ -88,11 +104,11 @@ class GnrInputGrads(C.Structure):
 EXPORTS = ("gnr_abi_version", "gnr_build_info", "gnr_set_conv16_tile", "gnr_sizeof", "gnr_workspace_bytes", "gnr_fwd", "gnr_fwd_bf16x3", "gnr_bwd", "gnr_bwd_bf16x3", "gnr_resample",
            "gnr_sample_zvals", "gnr_set_kernel_timing", "gnr_set_aux_timing", "gnr_set_stage_timing", "gnr_set_clock_probe", "gnr_merge_scratch_bytes",
            "gnr_merge_fwd", "gnr_merge_bwd", "gnr_upsample_workspace_bytes", "gnr_upsample_fwd", "gnr_upsample_bwd",
-           "gnr_last_error")
+           "gnr_quantize_rows", "gnr_read_rows", "gnr_int8_linear_workspace_bytes", "gnr_int8_linear", "gnr_last_error")
 
 # order == the GNR_SIZEOF_* ids of include/gnr.h
 STRUCTS = (GnrProblem, GnrWeights, GnrOutputs, GnrOutputGrads, GnrInputGrads, GnrMergeProblem, GnrUpsampleProblem,
-           GnrUpsampleWeights)
+           GnrUpsampleWeights, GnrRowsProblem, GnrInt8Problem)
 
 _lib = None
 
@@ -195,6 +211,13 @@ def load():
     lib.gnr_set_clock_probe.argtypes = [_p]
     lib.gnr_set_aux_timing.restype = C.c_int
     lib.gnr_set_aux_timing.argtypes = [_p, _p]
+    for name in ("gnr_quantize_rows", "gnr_read_rows"):
+        getattr(lib, name).restype = C.c_int
+        getattr(lib, name).argtypes = [C.POINTER(GnrRowsProblem), _p]
+    lib.gnr_int8_linear_workspace_bytes.restype = C.c_size_t
+    lib.gnr_int8_linear_workspace_bytes.argtypes = [C.POINTER(GnrInt8Problem)]
+    lib.gnr_int8_linear.restype = C.c_int
+    lib.gnr_int8_linear.argtypes = [C.POINTER(GnrInt8Problem), _p, C.c_size_t, _p]
     lib.gnr_sizeof.restype = C.c_size_t
     lib.gnr_sizeof.argtypes = [C.c_int]
     for which, cls in enumerate(STRUCTS):

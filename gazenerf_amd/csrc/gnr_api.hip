@@ -262,6 +262,8 @@ size_t gnr_sizeof(int which) {
         case GNR_SIZEOF_MERGE_PROBLEM: return sizeof(GnrMergeProblem);
         case GNR_SIZEOF_UPSAMPLE_PROBLEM: return sizeof(GnrUpsampleProblem);
         case GNR_SIZEOF_UPSAMPLE_WEIGHTS: return sizeof(GnrUpsampleWeights);
+        case GNR_SIZEOF_ROWS_PROBLEM: return sizeof(GnrRowsProblem);
+        case GNR_SIZEOF_INT8_PROBLEM: return sizeof(GnrInt8Problem);
         default: return 0;
     }
 }

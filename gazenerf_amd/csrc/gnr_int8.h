@@ -1,0 +1,82 @@
+// gnr_int8.h -- what gnr_quant.hip (8-bit rows: quantise, cache write, cache read) and gnr_int8.hip (their product) share.
+//
+// A ROW is the channel vector of one pixel (or one token): K signed bytes, contiguous, and ONE fp32 scale:
+//     a = max(max_k |x_k|, 2^-100)      scale = a / 127      q_k = rint(fl32(x_k * fl32(127 / a)))
+// The two roundings to fp32 belong to the definition (a value on the border between two steps has one answer).  |q| <= 127:
+// x_k / a <= 1 and 127 * (1 + 2^-23) still rounds to 127.  The floor 2^-100 keeps 127 / a finite; an all-zero row has q = 0.
+// A row that holds an Inf or a NaN gets q = 0 and scale = NaN: it reads back as NaN, in products too.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "../../include/gnr.h"
+
+namespace gnr {
+int fail(const char* fmt, ...);
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef float fv4 __attribute__((ext_vector_type(4)));
+
+constexpr unsigned ROW_FLOOR_BITS = 0x0d800000u;        // 2^-100
+
+// Elements of 16 consecutive bytes.  The pointers need the element's own alignment only: gfx950 loads and stores 16 bytes
+// at any address (rows of 129 halves or 387 floats start anywhere), so no path is split on alignment.
+template <typename T> struct Vec {
+    static constexpr int N = 16 / sizeof(T);
+    T v[N];
+};
+template <typename T> __device__ __forceinline__ Vec<T> load_vec(const T* p) {
+    Vec<T> r;
+    __builtin_memcpy(&r, p, 16);
+    return r;
+}
+// n < N elements (none for n <= 0), the rest 0
+template <typename T> __device__ __forceinline__ Vec<T> load_part(const T* p, int n) {
+    if (n >= Vec<T>::N) return load_vec(p);
+    Vec<T> r;
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i) r.v[i] = i < n ? p[i] : (T)0.0f;
+    return r;
+}
+template <typename T> __device__ __forceinline__ void store_part(T* p, const Vec<T>& r, int n) {
+    if (n >= Vec<T>::N) {
+        __builtin_memcpy(p, &r, 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < Vec<T>::N; ++i)
+            if (i < n) p[i] = r.v[i];
+    }
+}
+
+__device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }   // ordered like |x|; Inf, NaN on top
+
+// the row's scale and its reciprocal step from the largest abs_bits(); a row with an Inf / NaN: per = 0, scale = NaN
+__device__ __forceinline__ void row_scale(unsigned a_bits, float& scale, float& per) {
+    const bool bad = a_bits >= 0x7f800000u;
+    const float a = __uint_as_float(a_bits > ROW_FLOOR_BITS ? a_bits : ROW_FLOOR_BITS);
+    scale = bad ? __uint_as_float(0x7fc00000u) : a / 127.0f;
+    per = bad ? 0.0f : 127.0f / a;
+}
+// per == 0 marks a bad row: its values may be Inf / NaN, whose product is NaN -> q = 0
+__device__ __forceinline__ int row_step(float x, float per) { return per == 0.0f ? 0 : (int)rintf(x * per); }
+__device__ __forceinline__ unsigned pack4(int a, int b, int c, int d) {
+    return (unsigned)(a & 255) | (unsigned)(b & 255) << 8 | (unsigned)(c & 255) << 16 | (unsigned)d << 24;
+}
+
+// Where row `i` of a slot list lives.  slots == NULL: i itself.  A negative slot is padding (an empty row), a slot beyond the
+// cache a mistake: neither is addressed, the caller gets base 0 and the scale that stands for it (0 / NaN).
+struct SlotRef {
+    long slot;
+    int state;        // 0: in the cache; 1: padding; 2: out of range
+};
+__device__ __forceinline__ SlotRef slot_of(const int64_t* slots, long n_slots, long i) {
+    if (!slots) return SlotRef{i, 0};
+    const long s = slots[i];
+    return s < 0 ? SlotRef{0, 1} : (s >= n_slots ? SlotRef{0, 2} : SlotRef{s, 0});
+}
+
+int check_rows(const GnrRowsProblem* p, const char* what);
+int launch_quantize(const GnrRowsProblem& p, hipStream_t st);        // defined in gnr_quant.hip; 0 == enqueued
+}  // namespace gnr

@@ -258,6 +258,224 @@ int64_t saved_workspace_bytes(int64_t batch, int64_t n_rays, int64_t n_samples, 
     return (int64_t)n;
 }
 
+
+// ---- 8-bit rows (gazenerf_amd/int8.py documents the operators) ------------------------------------------------------------------
+int type_id(at::ScalarType t, const char* name) {
+    switch (t) {
+        case at::kFloat: return GNR_F32;
+        case at::kBFloat16: return GNR_BF16;
+        case at::kHalf: return GNR_F16;
+        default: TORCH_CHECK(false, name, " must be float32, bfloat16 or float16, got ", t);
+    }
+    return -1;
+}
+at::ScalarType type_of(int64_t id) {
+    TORCH_CHECK(id == GNR_F32 || id == GNR_BF16 || id == GNR_F16, "unknown type id ", id);
+    return id == GNR_F32 ? at::kFloat : (id == GNR_BF16 ? at::kBFloat16 : at::kHalf);
+}
+void check_on(const Tensor& t, const char* name, at::ScalarType type, int64_t dims, const c10::Device& dev) {
+    TORCH_CHECK(t.defined() && t.device() == dev, name, " must live on ", dev);
+    TORCH_CHECK(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
+    TORCH_CHECK(dims < 0 || t.dim() == dims, name, " must have ", dims, " dimensions, got shape ", t.sizes());
+}
+void check_cuda(const Tensor& t, const char* name) {
+    TORCH_CHECK(t.defined() && t.is_cuda(), name, " must live on a CUDA/ROCm device (the 8-bit operators have no CPU path)");
+}
+int64_t row_pitch(int64_t k) { return (k + 15) / 16 * 16; }
+Tensor empty_rows(int64_t b, int64_t n, int64_t k, const c10::Device& dev) {
+    Tensor t = at::empty({b, n, row_pitch(k)}, at::TensorOptions().dtype(at::kChar).device(dev));
+    return t.slice(2, 0, k);
+}
+// [B, C, ...] -> [B, C, P], [..., K] -> [b, n, K]: views, or copies where the strides need them
+Tensor maps3(const Tensor& t) {
+    TORCH_CHECK(t.dim() >= 3, "maps must be [B, C, ...], got ", t.sizes());
+    Tensor m = t;
+    if (t.dim() != 3) {
+        int64_t pix = 1;
+        for (int64_t d = 2; d < t.dim(); ++d) pix *= t.size(d);
+        m = t.reshape({t.size(0), t.size(1), pix});
+    }
+    return m.stride(2) == 1 || m.size(2) <= 1 ? m : m.contiguous();
+}
+Tensor rows3(const Tensor& t) {
+    TORCH_CHECK(t.dim() >= 1, "rows must be [..., K]");
+    const int64_t k = t.size(-1);
+    Tensor m = t;
+    if (t.dim() == 2) {
+        m = t.unsqueeze(0);
+    } else if (t.dim() != 3) {
+        int64_t n = 1;
+        for (int64_t d = 0; d + 1 < t.dim(); ++d) n *= t.size(d);
+        m = t.reshape({1, n, k});
+    }
+    return m.stride(2) == 1 || k <= 1 ? m : m.contiguous();
+}
+int64_t stride_or(const Tensor& t, int64_t d, int64_t other) { return t.size(d) > 1 ? t.stride(d) : other; }
+// 8-bit rows [b, n, K] as a product reads them: on 16-byte boundaries, readable to the next multiple of 16
+Tensor pitched(const Tensor& q) {
+    const int64_t b = q.size(0), n = q.size(1), k = q.size(2), k16 = row_pitch(k);
+    bool ok = (k == 1 || q.stride(2) == 1) && (n <= 1 || (q.stride(1) % 16 == 0 && q.stride(1) >= k16)) &&
+              (b <= 1 || q.stride(0) % 16 == 0) && (uintptr_t)q.data_ptr() % 16 == 0;
+    if (ok && q.numel() != 0) {
+        const int64_t last = q.storage_offset() + (b - 1) * q.stride(0) + (n - 1) * q.stride(1) + k16;
+        ok = last <= (int64_t)q.storage().nbytes();
+    }
+    if (ok) return q;
+    Tensor out = empty_rows(b, n, k, q.device());
+    out.copy_(q);
+    return out;
+}
+void* stream_of(const c10::Device& dev) { return (void*)c10::hip::getCurrentHIPStream(dev.index()).stream(); }
+
+GnrRowsProblem rows_problem(const Tensor& x3, bool cf, const Tensor& q, const Tensor& scale) {
+    GnrRowsProblem p = GNR_INIT_ROWS_PROBLEM;
+    p.dtype = type_id(x3.scalar_type(), "x"); p.channels_first = cf;
+    TORCH_CHECK(x3.size(0) <= INT32_MAX && x3.size(cf ? 1 : 2) <= INT32_MAX, "too many maps or channels: ", x3.sizes());
+    p.batch = (int32_t)x3.size(0); p.channels = (int32_t)x3.size(cf ? 1 : 2); p.n_pix = x3.size(cf ? 2 : 1);
+    p.x = x3.data_ptr(); p.x_batch = x3.stride(0); p.x_stride = x3.stride(1);
+    p.q = (int8_t*)q.data_ptr(); p.q_batch = q.stride(0); p.q_pitch = stride_or(q, 1, row_pitch(q.size(2)));
+    p.scale = scale.data_ptr<float>(); p.scale_batch = scale.stride(0);
+    return p;
+}
+
+std::vector<Tensor> quantize_rows(const Tensor& x, bool cf) {
+    check_cuda(x, "x");
+    type_id(x.scalar_type(), "x");
+    const c10::DeviceGuard guard(x.device());
+    const Tensor x3 = cf ? maps3(x) : rows3(x);
+    const int64_t b = x3.size(0), n = x3.size(cf ? 2 : 1), k = x3.size(cf ? 1 : 2);
+    TORCH_CHECK(k >= 1, "x has no channels: ", x.sizes());
+    Tensor q = empty_rows(b, n, k, x.device()), scale = at::empty({b, n}, at::TensorOptions().dtype(at::kFloat).device(x.device()));
+    if (x3.numel() != 0) {
+        const GnrRowsProblem p = rows_problem(x3, cf, q, scale);
+        check_rc(gnr_quantize_rows(&p, stream_of(x.device())));
+    }
+    if (!cf && x.dim() != 3) {
+        std::vector<int64_t> lead(x.sizes().begin(), x.sizes().end() - 1), shape(x.sizes().begin(), x.sizes().end()), strides(shape.size(), 1);
+        int64_t s = row_pitch(k);
+        for (size_t d = lead.size(); d-- > 0;) { strides[d] = s; s *= lead[d]; }
+        q = q.as_strided(shape, strides);
+        scale = scale.view(lead);
+    }
+    return {q, scale};
+}
+
+void check_cache(const Tensor& q, const Tensor& scale, const Tensor& slots) {
+    check_cuda(q, "q");
+    check_on(q, "q", at::kChar, 3, q.device());
+    check_on(scale, "scale", at::kFloat, 2, q.device());
+    check_on(slots, "slots", at::kLong, 1, q.device());
+    const int64_t n = q.size(0), p = q.size(1), c = q.size(2);
+    TORCH_CHECK(n >= 1 && p >= 1 && c >= 1, "the cache is empty: q ", q.sizes());
+    TORCH_CHECK(scale.size(0) == n && scale.size(1) == p, "scale must have shape [", n, ", ", p, "], got ", scale.sizes());
+    TORCH_CHECK((c == 1 || q.stride(2) == 1) && (p == 1 || q.stride(1) >= c) && (n == 1 || q.stride(0) >= (p - 1) * q.stride(1) + c),
+                "q must have its channels contiguous and its rows apart, got strides ", q.strides());
+    TORCH_CHECK((p == 1 || scale.stride(1) == 1) && (n == 1 || scale.stride(0) >= p),
+                "scale must have its pixels contiguous and its slots apart, got strides ", scale.strides());
+}
+
+void write_featmaps(const Tensor& q, const Tensor& scale, const Tensor& slots, const Tensor& maps) {
+    check_cache(q, scale, slots);
+    TORCH_CHECK(maps.defined() && maps.device() == q.device(), "maps must live on ", q.device());
+    type_id(maps.scalar_type(), "maps");
+    const c10::DeviceGuard guard(q.device());
+    const Tensor m = maps3(maps), sl = slots.contiguous();
+    TORCH_CHECK(m.size(0) == sl.size(0) && m.size(1) == q.size(2) && m.size(2) == q.size(1), "maps must be [", sl.size(0), ", ", q.size(2),
+                ", ...] with ", q.size(1), " pixels, got ", maps.sizes());
+    if (m.numel() == 0) return;
+    GnrRowsProblem p = rows_problem(m, true, q, scale);
+    p.slots = sl.data_ptr<int64_t>(); p.n_slots = q.size(0);
+    check_rc(gnr_quantize_rows(&p, stream_of(q.device())));
+}
+
+Tensor read_featmaps(const Tensor& q, const Tensor& scale, const Tensor& slots, int64_t out_type) {
+    check_cache(q, scale, slots);
+    const c10::DeviceGuard guard(q.device());
+    const Tensor sl = slots.contiguous();
+    Tensor out = at::empty({sl.size(0), q.size(2), q.size(1)}, at::TensorOptions().dtype(type_of(out_type)).device(q.device()));
+    if (out.numel() == 0) return out;
+    GnrRowsProblem p = rows_problem(out, true, q, scale);
+    p.slots = sl.data_ptr<int64_t>(); p.n_slots = q.size(0);
+    check_rc(gnr_read_rows(&p, stream_of(q.device())));
+    return out;
+}
+
+Tensor int8_linear(const Tensor& x, const Tensor& w_q, const Tensor& w_scale, const OptTensor& bias, const OptTensor& x_scale,
+                   const OptTensor& slots, bool leaky, bool cf, int64_t out_type) {
+    check_cuda(x, "x");
+    const c10::Device dev = x.device();
+    const c10::DeviceGuard guard(dev);
+    const bool rows8 = x.scalar_type() == at::kChar;
+    check_on(w_q, "w_q", at::kChar, 2, dev);
+    check_on(w_scale, "w_scale", at::kFloat, 1, dev);
+    const int64_t o = w_q.size(0), k = w_q.size(1);
+    TORCH_CHECK(o >= 1 && k >= 1 && o <= INT32_MAX && k <= GNR_INT8_MAX_K, "w_q has a shape the product cannot take: ", w_q.sizes());
+    TORCH_CHECK(w_scale.size(0) == o, "w_scale must have shape [", o, "], got ", w_scale.sizes());
+    GnrInt8Problem p = GNR_INIT_INT8_PROBLEM;
+    p.x_type = rows8 ? GNR_I8 : type_id(x.scalar_type(), "x");
+    const at::ScalarType yt = type_of(out_type);
+    p.y_type = (int32_t)out_type; p.leaky = leaky; p.y_channels_first = cf; p.k = (int32_t)k; p.o = (int32_t)o;
+    const Tensor w = pitched(w_q.unsqueeze(0)), ws_c = w_scale.contiguous();
+    Tensor b_c, xr, xs, sl;
+    if (bias) {
+        check_on(*bias, "bias", at::kFloat, 1, dev);
+        TORCH_CHECK(bias->size(0) == o, "bias must have shape [", o, "], got ", bias->sizes());
+        b_c = bias->contiguous();
+    }
+    int64_t b, n;
+    std::vector<int64_t> shape;
+    if (rows8) {
+        TORCH_CHECK(x_scale, "8-bit x needs its x_scale");
+        TORCH_CHECK(x.dim() >= 1 && x.size(-1) == k, "x has another number of channels than w_q: ", x.sizes(), ", ", w_q.sizes());
+        TORCH_CHECK((!slots && !cf) || x.dim() == 3, "with slots or channels_first, 8-bit x must be [n, P, K], got ", x.sizes());
+        check_on(*x_scale, "x_scale", at::kFloat, x.dim() - 1, dev);
+        TORCH_CHECK(x_scale->sizes() == x.sizes().slice(0, x.dim() - 1), "x_scale must have the shape of x without its channels, got ",
+                    x_scale->sizes());
+        xr = pitched(rows3(x));
+        b = xr.size(0); n = xr.size(1);
+        xs = x.dim() == 3 ? *x_scale : x_scale->reshape({b, n});
+        if (xs.size(1) > 1 && xs.stride(1) != 1) xs = xs.contiguous();
+        p.x_scale = xs.data_ptr<float>(); p.x_scale_batch = xs.stride(0);
+        p.x_batch = stride_or(xr, 0, 0); p.x_stride = stride_or(xr, 1, row_pitch(k));
+        if (slots) {
+            check_on(*slots, "slots", at::kLong, 1, dev);
+            TORCH_CHECK(b >= 1, "slots are given but x is empty: ", x.sizes());
+            sl = slots->contiguous();
+            p.slots = sl.data_ptr<int64_t>(); p.n_slots = b;
+            b = sl.size(0);
+        }
+        if (cf) shape = {b, o, n};
+        else if (slots) shape = {b, n, o};
+    } else {
+        TORCH_CHECK(!x_scale && !slots, "x_scale and slots go with 8-bit x; floating x is quantised by the call");
+        xr = cf ? maps3(x) : rows3(x);
+        b = xr.size(0); n = xr.size(cf ? 2 : 1);
+        TORCH_CHECK(xr.size(cf ? 1 : 2) == k, "x has another number of channels than w_q: ", x.sizes(), ", ", w_q.sizes());
+        p.x_channels_first = cf; p.x_batch = xr.stride(0); p.x_stride = xr.stride(1);
+        if (cf) {
+            shape = x.sizes().vec();
+            shape[1] = o;
+        }
+    }
+    if (shape.empty()) {
+        shape = x.sizes().vec();
+        shape.back() = o;
+    }
+    Tensor y = at::empty(shape, at::TensorOptions().dtype(yt).device(dev));
+    if (y.numel() == 0) return y;
+    TORCH_CHECK(b <= INT32_MAX, "too many entries: ", b);
+    p.batch = (int32_t)b; p.n_pix = n; p.x = xr.data_ptr();
+    p.w = (const int8_t*)w.data_ptr(); p.w_pitch = stride_or(w, 1, row_pitch(k)); p.w_scale = ws_c.data_ptr<float>();
+    p.bias = bias ? b_c.data_ptr<float>() : nullptr;
+    p.y = y.data_ptr();
+    const size_t need = gnr_int8_linear_workspace_bytes(&p);
+    TORCH_CHECK(need != 0, gnr_last_error());
+    Tensor ws;
+    if (!rows8) ws = alloc_ws(need, dev);
+    check_rc(gnr_int8_linear(&p, rows8 ? nullptr : ws.data_ptr(), rows8 ? 0 : (size_t)ws.numel(), stream_of(dev)));
+    return y;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -270,5 +488,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("build_info", []() { return std::string(gnr_build_info()); }, "gnr_build_info() of the libgnr.so it is linked to");
     m.def("render_fwd", &render_fwd, "gnr_fwd / gnr_fwd_bf16x3 on the current HIP stream");
     m.def("render_bwd", &render_bwd, "gnr_bwd / gnr_bwd_bf16x3 on the current HIP stream");
+    m.def("quantize_rows", &quantize_rows, "gnr_quantize_rows on the current HIP stream -> [q, scale]");
+    m.def("write_featmaps", &write_featmaps, "gnr_quantize_rows into the slots of a cache");
+    m.def("read_featmaps", &read_featmaps, "gnr_read_rows from the slots of a cache");
+    m.def("int8_linear", &int8_linear, "gnr_int8_linear on the current HIP stream");
     m.def("saved_workspace_bytes", &saved_workspace_bytes, "bytes of saved activations for a training forward of this size");
 }

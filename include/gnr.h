@@ -171,7 +171,7 @@ int gnr_abi_version(void);
  * own declarations at load time (the ctypes binding does).  Unknown id -> 0. */
 enum { GNR_SIZEOF_PROBLEM = 0, GNR_SIZEOF_WEIGHTS = 1, GNR_SIZEOF_OUTPUTS = 2, GNR_SIZEOF_OUTPUT_GRADS = 3,
        GNR_SIZEOF_INPUT_GRADS = 4, GNR_SIZEOF_MERGE_PROBLEM = 5, GNR_SIZEOF_UPSAMPLE_PROBLEM = 6,
-       GNR_SIZEOF_UPSAMPLE_WEIGHTS = 7 };
+       GNR_SIZEOF_UPSAMPLE_WEIGHTS = 7, GNR_SIZEOF_ROWS_PROBLEM = 8, GNR_SIZEOF_INT8_PROBLEM = 9 };
 size_t gnr_sizeof(int which);
 
 /* Bytes of workspace `kind` needs for problem `p` with `n_streams` (1 or 2) weight sets. */
@@ -324,6 +324,70 @@ int gnr_upsample_fwd(const GnrUpsampleProblem* p, const GnrUpsampleWeights* w, f
 int gnr_upsample_bwd(const GnrUpsampleProblem* p, const GnrUpsampleWeights* w, const float* d_img, float* d_x,
                      const GnrUpsampleWeightGrads* dw, void* saved_workspace, size_t saved_bytes, void* scratch,
                      size_t scratch_bytes, void* stream);
+
+/* ---- 8-bit rows: feature maps kept in 8 bits, and the 1x1 convolutions / linear layers that read them -------------------------
+ * A ROW is the channel vector of one pixel (one token): `channels` signed bytes and one fp32 scale,
+ *     a = max(max_k |x_k|, 2^-100)     scale = a / 127     q_k = rint(fl32(x_k * fl32(127 / a)))         (ties to even)
+ * A row that holds an Inf or a NaN gets q = 0, scale = NaN and reads back as NaN.  Inference only: no gradients. */
+enum { GNR_F32 = 0, GNR_BF16 = 1, GNR_F16 = 2, GNR_I8 = 3 };
+
+typedef struct GnrRowsProblem {
+    uint32_t struct_size;       /* = sizeof(GnrRowsProblem) of the caller                                        */
+    int32_t dtype;              /* of x: GNR_F32, GNR_BF16, GNR_F16                                              */
+    int32_t channels_first;     /* x: 1 = maps, element (b, c, i) at x[b x_batch + c x_stride + i];
+                                      0 = rows, element (b, i, c) at x[b x_batch + i x_stride + c]  (in elements) */
+    int32_t batch;              /* entries (maps) of x; 0 is an empty call                                       */
+    int64_t n_pix;              /* rows of an entry                                                              */
+    int32_t channels;
+    int32_t reserved;
+    void* x;
+    int64_t x_batch, x_stride;
+    int8_t* q;                  /* row (s, i) at q + s q_batch + i q_pitch (bytes), s = slots[b] or b            */
+    int64_t q_batch, q_pitch;
+    float* scale;               /* scale (s, i) at scale[s scale_batch + i]                                      */
+    int64_t scale_batch;
+    const int64_t* slots;       /* device, [batch], or NULL.  A negative slot is padding: nothing is written, zeros are read.
+                                   A slot >= n_slots: nothing is written, NaN is read (it is never addressed).   */
+    int64_t n_slots;
+} GnrRowsProblem;
+#define GNR_INIT_ROWS_PROBLEM { (uint32_t)sizeof(GnrRowsProblem) }
+
+/* x -> rows.  With slots (channels_first only): the maps go into those slots of a cache; of several maps with the same slot the LAST
+ * one of the list stays.  Bytes behind a row's channels and slots that are not named are left as they are.  n_pix * batch <= 2^31. */
+int gnr_quantize_rows(const GnrRowsProblem* p, void* stream);
+/* rows -> x (channels_first only): q * scale rounded to dtype. */
+int gnr_read_rows(const GnrRowsProblem* p, void* stream);
+
+/* y(b, i, o) = act((sum_k x_q w_q) * x_scale(b, i) * w_scale(o) + bias(o)): a linear layer over rows, i.e. a 1x1 convolution over
+ * the pixels of maps.  The sum is exact; the epilogue is fp32; y is rounded once. */
+#define GNR_INT8_MAX_K 131071
+typedef struct GnrInt8Problem {
+    uint32_t struct_size;       /* = sizeof(GnrInt8Problem) of the caller                                        */
+    int32_t x_type;             /* GNR_I8: rows as gnr_quantize_rows writes them; a floating type: quantised by the call */
+    int32_t y_type;             /* GNR_F32, GNR_BF16, GNR_F16                                                    */
+    int32_t leaky;              /* LeakyReLU(0.2) behind the bias                                                */
+    int32_t x_channels_first;   /* floating x only: maps instead of rows (GnrRowsProblem)                        */
+    int32_t y_channels_first;   /* y [batch][o][n_pix] instead of [batch][n_pix][o]; contiguous                  */
+    int32_t batch, k, o, reserved;
+    int64_t n_pix;
+    const void* x;
+    int64_t x_batch, x_stride;  /* strides as in GnrRowsProblem, in elements.  GNR_I8: x 16-byte aligned, both multiples of 16,
+                                   every row readable up to the next multiple of 16 behind k (those bytes count as 0)     */
+    const float* x_scale;       /* GNR_I8: scale (s, i) at x_scale[s x_scale_batch + i]                          */
+    int64_t x_scale_batch;
+    const int64_t* slots;       /* GNR_I8: device, [batch], or NULL: x is a cache of n_slots entries and entry b is slots[b].
+                                   A negative slot is an entry of zero rows; a slot >= n_slots gives NaN         */
+    int64_t n_slots;
+    const int8_t* w;            /* [o] rows of k bytes on w_pitch (16-byte aligned, multiple of 16, readable like x) */
+    int64_t w_pitch;
+    const float* w_scale;       /* [o]                                                                           */
+    const float* bias;          /* [o] or NULL                                                                   */
+    void* y;
+} GnrInt8Problem;
+#define GNR_INIT_INT8_PROBLEM { (uint32_t)sizeof(GnrInt8Problem) }
+
+size_t gnr_int8_linear_workspace_bytes(const GnrInt8Problem* p);     /* 0 + gnr_last_error() on bad input */
+int gnr_int8_linear(const GnrInt8Problem* p, void* workspace, size_t ws_bytes, void* stream);
 
 const char* gnr_last_error(void);
 
