@@ -8,17 +8,29 @@
 
 namespace gnr {
 
+// Workgroups go round robin over the 8 XCDs: block i works on tile (i % 8) (n / 8) + i / 8, so that one XCD walks neighbouring tiles
+__device__ __forceinline__ unsigned xcd_block(unsigned n) {
+    const unsigned per = n >> 3;
+    return blockIdx.x < per * 8 ? (blockIdx.x & 7) * per + (blockIdx.x >> 3) : blockIdx.x;
+}
+__device__ __forceinline__ long tile_start(unsigned i, int tp, long n) {
+    const long p = (long)i * tp;
+    return p + tp <= n || n < tp ? p : n - tp;
+}
+
 // ---------------------------------------------------------------------------------------------
-// channels-first maps [B][C][P] -> rows.  8 lanes x 16 bytes cover the tile's pixels of one channel (128 bytes: a whole line), a
-// thread keeps R quads of channels in registers between the row maximum and the quantisation, so x is read once up to 2048
-// channels (1024 threads, R = 4); wider rows are read twice.
+// channels-first maps [B][C][P] -> rows.  A tile is 32 pixels: LPX lanes x 16 bytes cover them in one channel (a line of 128 bytes in
+// fp32), a thread keeps R quads of channels in registers between the row maximum and the quantisation, so x is read once up to
+// 2048 channels (fp32; 4096 in 16 bits: 1024 threads, R = 4); wider rows are read twice.  Bound by memory: 64 maps of 258 x 4096 in
+// fp32 (339 MB) take 78 us = 4.3 TB/s, 16 maps of 1024 x 4096 in fp16 (202 MB) 44 us = 4.6 TB/s; a large copy on this card: 4.7.
 // ---------------------------------------------------------------------------------------------
-template <typename T, int R>
-__global__ __launch_bounds__(1024) void quant_maps_kernel(const GnrRowsProblem p, unsigned tiles) {
-    constexpr int V = Vec<T>::N, TP = 8 * V;
+template <typename T, int LPX, int R>
+__global__ __launch_bounds__(1024) void quant_maps_kernel(const GnrRowsProblem p, unsigned tiles, int ld) {
+    constexpr int V = Vec<T>::N, TP = LPX * V;
     extern __shared__ unsigned smem[];
-    const int NT = (int)blockDim.x, G = NT >> 3, tid = (int)threadIdx.x, l = tid & 7, g = tid >> 3;
-    const long b = blockIdx.x / tiles, p0 = (long)(blockIdx.x % tiles) * TP;
+    const int NT = (int)blockDim.x, G = NT / LPX, tid = (int)threadIdx.x, l = tid % LPX, g = tid / LPX;
+    const unsigned at = xcd_block(gridDim.x);
+    const long b = at / tiles, p0 = tile_start(at % tiles, TP, p.n_pix);
     long slot = b;
     if (p.slots) {
         const SlotRef ref = slot_of(p.slots, p.n_slots, b);
@@ -29,25 +41,29 @@ __global__ __launch_bounds__(1024) void quant_maps_kernel(const GnrRowsProblem p
         for (long j = b + 1 + tid; j < p.batch; j += NT) again |= p.slots[j] == slot;
         if (__syncthreads_or(again)) return;
     }
-    unsigned* tile = smem;                                  // [TP][G + 4]: one quad of channels of one pixel a word
-    unsigned* amax = smem + TP * (G + 4);                   // [NT / 64][TP]
-    const int C = p.channels, ld = G + 4;
-    const T* xb = (const T*)p.x + b * p.x_batch + p0 + l * V;
-    const long left = p.n_pix - p0 - l * V;
-    const int nv = left >= V ? V : (left > 0 ? (int)left : 0);
+    unsigned* tile = smem;                                  // [TP][ld]: one quad of channels of one pixel a word
+    unsigned* amax = smem + TP * ld;                        // [NT / 64][LPX][4]
+    const int C = p.channels;
+    // a tile that would reach over the map's end moves back to end with it, and so do the lanes of a map smaller than a tile: some
+    // pixels are done twice, with the same results, and every access is a whole vector unless the map itself is smaller
+    const bool whole = p.n_pix >= V;
+    const long pl = whole ? (p0 + l * V < p.n_pix - V ? p0 + l * V : p.n_pix - V) : 0;
+    const int nv = whole ? V : (int)p.n_pix;
+    const T* xb = (const T*)p.x + b * p.x_batch + pl;
     const int step = 4 * G * R, n_chunk = (C + step - 1) / step;
 
-    Vec<T> x[R][4];
+    Raw16 x[R][4];
     auto load = [&](int c0) {
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int c = c0 + 4 * (r * G + g) + e;
-                x[r][e] = load_part(xb + (long)(c < C ? c : 0) * p.x_stride, c < C ? nv : 0);
+                if (c < C) x[r][e] = load_raw(xb + (long)c * p.x_stride, nv);
+                else x[r][e] = Raw16{};
             }
     };
-    unsigned a[V] = {};
+    unsigned a[4] = {};
     for (int k = 0; k < n_chunk; ++k) {
         load(k * step);
 #pragma unroll
@@ -55,54 +71,48 @@ __global__ __launch_bounds__(1024) void quant_maps_kernel(const GnrRowsProblem p
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const unsigned u = abs_bits((float)x[r][e].v[v]);
-                    a[v] = u > a[v] ? u : a[v];
-                }
+                for (int w = 0; w < 4; ++w) a[w] = max_bits<T>(a[w], x[r][e].w[w]);
     }
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
+    for (int w = 0; w < 4; ++w) {
 #pragma unroll
-        for (int m = 8; m < 64; m <<= 1) {
-            const unsigned u = (unsigned)__shfl_xor((int)a[v], m);
-            a[v] = u > a[v] ? u : a[v];
-        }
-        if ((tid & 63) < 8) amax[(tid >> 6) * TP + l * V + v] = a[v];
+        for (int m = LPX; m < 64; m <<= 1) a[w] = max_bits<T>(a[w], (unsigned)__shfl_xor((int)a[w], m));
+        if ((tid & 63) < LPX) amax[((tid >> 6) * LPX + l) * 4 + w] = a[w];
     }
     __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+        for (int i = 0; i < NT >> 6; ++i) a[w] = max_bits<T>(a[w], amax[(i * LPX + l) * 4 + w]);
     float per[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        unsigned m = 0;
-        for (int w = 0; w < NT >> 6; ++w) {
-            const unsigned u = amax[w * TP + l * V + v];
-            m = u > m ? u : m;
-        }
         float s;
-        row_scale(m, s, per[v]);
-        if (g == 0 && v < nv) p.scale[slot * p.scale_batch + p0 + l * V + v] = s;
+        row_scale(__float_as_uint(raw_value<T>(a, v)), s, per[v]);
+        if (g == 0 && v < nv) p.scale[slot * p.scale_batch + pl + v] = s;
     }
-    int8_t* qb = p.q + slot * p.q_batch + p0 * p.q_pitch;
+    int8_t* qb = p.q + slot * p.q_batch;
+    const int rows = p.n_pix - p0 < TP ? (int)(p.n_pix - p0) : TP;
+    const int shift = (int)(pl - p0);                       // this lane's first row in the tile
     for (int k = 0; k < n_chunk; ++k) {
-        if (n_chunk > 1) load(k * step);
+        if (n_chunk > 1) {
+            load(k * step);
+            __syncthreads();
+        }
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
+        for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int v = 0; v < V; ++v)
-                tile[(l * V + v) * ld + g] =
-                    pack4(row_step((float)x[r][0].v[v], per[v]), row_step((float)x[r][1].v[v], per[v]),
-                          row_step((float)x[r][2].v[v], per[v]), row_step((float)x[r][3].v[v], per[v]));
-            __syncthreads();
-            const int cr = k * step + 4 * r * G, per_row = G >> 2;          // 16-byte pieces of a row in this pass
-            for (int i = tid; i < TP * per_row; i += NT) {
-                const int row = i / per_row, c = cr + 16 * (i % per_row);
-                if (p0 + row < p.n_pix && c < C) {
-                    Vec<int8_t> o;
-                    __builtin_memcpy(&o, tile + row * ld + 4 * (i % per_row), 16);
-                    store_part(qb + (long)row * p.q_pitch + c, o, C - c);
-                }
-            }
-            __syncthreads();
+                if (v < nv && 4 * (k * G * R + r * G + g) < C)
+                    tile[(shift + v) * ld + r * G + g] =
+                        pack4(row_step(raw_value<T>(x[r][0].w, v), per[v]), row_step(raw_value<T>(x[r][1].w, v), per[v]),
+                              row_step(raw_value<T>(x[r][2].w, v), per[v]), row_step(raw_value<T>(x[r][3].w, v), per[v]));
+        __syncthreads();
+        const int c0 = k * step, cols = C - c0 < step ? C - c0 : step, per_row = (cols + 15) >> 4;      // 16-byte pieces of a row
+        for (int i = tid; i < rows * per_row; i += NT) {
+            const int row = i / per_row, c = 16 * (i - row * per_row);
+            Vec<int8_t> o;
+            __builtin_memcpy(&o, __builtin_assume_aligned(tile + row * ld + (c >> 2), 16), 16);
+            store_part(qb + (p0 + row) * p.q_pitch + c0 + c, o, cols - c);
         }
     }
 }
@@ -120,45 +130,43 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const GnrRowsProblem p,
     const T* x = (const T*)p.x + b * p.x_batch + pix * p.x_stride;
     int8_t* q = p.q + b * p.q_batch + pix * p.q_pitch;
     const int C = p.channels, step = L * J * V, n_chunk = (C + step - 1) / step;
-    Vec<T> r[J];
+    Raw16 r[J];
     auto load = [&](int c0) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             const int c = c0 + (j * L + lane) * V;
-            r[j] = load_part(x + (c < C ? c : 0), ok ? C - c : 0);
+            if (ok && c < C) r[j] = load_raw(x + (C < V ? 0 : (c < C - V ? c : C - V)), C);
+            else r[j] = Raw16{};
         }
     };
-    unsigned a = 0;
+    unsigned a[4] = {};
     for (int k = 0; k < n_chunk; ++k) {
         load(k * step);
 #pragma unroll
         for (int j = 0; j < J; ++j)
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const unsigned u = abs_bits((float)r[j].v[v]);
-                a = u > a ? u : a;
-            }
+            for (int w = 0; w < 4; ++w) a[w] = max_bits<T>(a[w], r[j].w[w]);
     }
+    a[0] = max_bits<T>(max_bits<T>(a[0], a[1]), max_bits<T>(a[2], a[3]));
 #pragma unroll
-    for (int m = 1; m < L; m <<= 1) {
-        const unsigned u = (unsigned)__shfl_xor((int)a, m);
-        a = u > a ? u : a;
-    }
+    for (int m = 1; m < L; m <<= 1) a[0] = max_bits<T>(a[0], (unsigned)__shfl_xor((int)a[0], m));
+    if constexpr (sizeof(T) == 2) a[0] = max_bits<T>(a[0], a[0] >> 16);
     float s, per;
-    row_scale(a, s, per);
+    row_scale(__float_as_uint(raw_value<T>(a, 0)), s, per);
     if (!ok) return;
     if (lane == 0) p.scale[b * p.scale_batch + pix] = s;
     for (int k = 0; k < n_chunk; ++k) {
         if (n_chunk > 1) load(k * step);
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int c = k * step + (j * L + lane) * V;
+            int c = k * step + (j * L + lane) * V;
             if (c >= C) continue;
+            if (C >= V && c > C - V) c = C - V;            // the last lane moves back: a few values twice, with the same results
             unsigned o[V / 4];
 #pragma unroll
             for (int w = 0; w < V / 4; ++w)
-                o[w] = pack4(row_step((float)r[j].v[4 * w], per), row_step((float)r[j].v[4 * w + 1], per),
-                             row_step((float)r[j].v[4 * w + 2], per), row_step((float)r[j].v[4 * w + 3], per));
+                o[w] = pack4(row_step(raw_value<T>(r[j].w, 4 * w), per), row_step(raw_value<T>(r[j].w, 4 * w + 1), per),
+                             row_step(raw_value<T>(r[j].w, 4 * w + 2), per), row_step(raw_value<T>(r[j].w, 4 * w + 3), per));
             if (c + V <= C) {
                 __builtin_memcpy(q + c, o, V);
             } else {
@@ -179,47 +187,51 @@ template <typename T> __device__ __forceinline__ T row_value(int q, float s) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// cached rows -> channels-first maps [B][C][P]: 128 channels of a tile of pixels pass through LDS at a time
+// cached rows -> channels-first maps [B][C][P].  A tile's rows go to LDS whole and ONE barrier later the workgroup only stores: with a
+// barrier per 128 channels every one of them waited for the stores before it.  The stores bypass the caches: four bytes leave for each
+// that came, and through the caches they push out the rows that the neighbouring tile is about to read.  64 maps of 258 x 4096, fp32
+// (339 MB): 112 us through the caches, 51 us = 6.6 TB/s past them.  (The tile -> XCD order of quant_maps_kernel costs here: 54 us.)
 // ---------------------------------------------------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(256) void read_maps_kernel(const GnrRowsProblem p, unsigned tiles) {
-    constexpr int V = Vec<T>::N, TP = 8 * V, G = 32, LD = G + 4, PIECES = TP * 8 / 256;
-    __shared__ unsigned tile[TP * LD];
-    const int tid = (int)threadIdx.x, l = tid & 7, g = tid >> 3;
-    const long b = blockIdx.x / tiles, p0 = (long)(blockIdx.x % tiles) * TP;
+template <typename T, int LPX>
+__global__ __launch_bounds__(256) void read_maps_kernel(const GnrRowsProblem p, unsigned tiles, int ld, int step) {
+    constexpr int V = Vec<T>::N, TP = LPX * V, G = 256 / LPX, U = 4;
+    extern __shared__ unsigned smem[];                      // [TP][ld]
+    const int tid = (int)threadIdx.x, l = tid % LPX, g = tid / LPX;
+    const unsigned at = blockIdx.x;
+    const long b = at / tiles, p0 = tile_start(at % tiles, TP, p.n_pix);
     const SlotRef ref = slot_of(p.slots, p.n_slots, b);
-    const int C = p.channels;
-    const int8_t* qb = p.q + ref.slot * p.q_batch;
-    const long left = p.n_pix - p0 - l * V;
-    const int nv = left >= V ? V : (left > 0 ? (int)left : 0);
+    const int C = p.channels, rows = p.n_pix - p0 < TP ? (int)(p.n_pix - p0) : TP;
+    const int8_t* qb = p.q + ref.slot * p.q_batch + p0 * p.q_pitch;
+    const bool whole = p.n_pix >= V;
+    const long pl = whole ? (p0 + l * V < p.n_pix - V ? p0 + l * V : p.n_pix - V) : 0;
+    const int nv = whole ? V : (int)p.n_pix, shift = (int)(pl - p0);
     float s[V];
 #pragma unroll
     for (int v = 0; v < V; ++v)
-        s[v] = ref.state ? (ref.state == 1 ? 0.0f : __uint_as_float(0x7fc00000u))
-                         : (v < nv ? p.scale[ref.slot * p.scale_batch + p0 + l * V + v] : 0.0f);
-    T* yb = (T*)p.x + b * p.x_batch + p0 + l * V;
-    for (int c0 = 0; c0 < C; c0 += 4 * G) {
+        s[v] = ref.state ? (ref.state == 1 ? 0.0f : __uint_as_float(0x7fc00000u)) : (v < nv ? p.scale[ref.slot * p.scale_batch + pl + v] : 0.0f);
+    T* yb = (T*)p.x + b * p.x_batch + pl;
+    for (int c0 = 0; c0 < C; c0 += step) {                  // once, unless the rows of a tile exceed the LDS
+        const int cols = C - c0 < step ? C - c0 : step, per_row = (cols + 15) >> 4, n = ref.state ? 0 : rows * per_row;
+        if (c0) __syncthreads();
+        for (int i0 = tid; i0 < n; i0 += 256 * U) {
+            Vec<int8_t> o[U];
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int row = (tid + 256 * i) >> 3, piece = tid & 7, c = c0 + 16 * piece;
-            Vec<int8_t> o = {};
-            if (!ref.state && p0 + row < p.n_pix && c < C) {
-                if (c + 16 <= C) {
-                    o = load_vec(qb + (p0 + row) * p.q_pitch + c);
-                } else {
-                    for (int e = 0; e < 16; ++e)
-                        if (c + e < C) o.v[e] = qb[(p0 + row) * p.q_pitch + c + e];
-                }
+            for (int u = 0; u < U; ++u) {
+                const int i = i0 + 256 * u, row = i / per_row, c = 16 * (i - row * per_row);
+                if (i < n) o[u] = load_part(qb + row * p.q_pitch + c0 + c, cols - c);
             }
-            __builtin_memcpy(tile + row * LD + 4 * piece, &o, 16);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = i0 + 256 * u, row = i / per_row, c = 16 * (i - row * per_row);
+                if (i < n) __builtin_memcpy(__builtin_assume_aligned(smem + row * ld + (c >> 2), 16), &o[u], 16);
+            }
         }
         __syncthreads();
-        const int c = c0 + 4 * g;
-        if (c < C && nv > 0) {
+        for (int q = g; 4 * q < cols; q += G) {
             Vec<T> y[4];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const int w = (int)tile[(l * V + v) * LD + g];
+                const int w = v < nv && !ref.state ? (int)smem[(shift + v) * ld + q] : 0;
                 y[0].v[v] = row_value<T>((int8_t)w, s[v]);
                 y[1].v[v] = row_value<T>((int8_t)(w >> 8), s[v]);
                 y[2].v[v] = row_value<T>((int8_t)(w >> 16), s[v]);
@@ -227,9 +239,8 @@ __global__ __launch_bounds__(256) void read_maps_kernel(const GnrRowsProblem p, 
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (c + e < C) store_part(yb + (long)(c + e) * p.x_stride, y[e], nv);
+                if (4 * q + e < cols) store_part<true>(yb + (long)(c0 + 4 * q + e) * p.x_stride, y[e], nv);
         }
-        __syncthreads();
     }
 }
 
@@ -254,21 +265,27 @@ int check_rows(const GnrRowsProblem* p, const char* what) {
     return 0;
 }
 
-template <typename T> static void quant_maps(const GnrRowsProblem& p, hipStream_t st) {
-    constexpr int TP = 8 * Vec<T>::N;
+template <typename T, int LPX> static void quant_maps_lpx(const GnrRowsProblem& p, int nt, hipStream_t st) {
+    constexpr int TP = LPX * Vec<T>::N;
     const unsigned tiles = (unsigned)((p.n_pix + TP - 1) / TP);
+    const int quads = (p.channels + 3) / 4, G = nt / LPX;
+    const int R = quads >= 4 * G ? 4 : (quads + G - 1) / G;
+    const int words = quads < G * R ? quads : G * R, ld = (words + 15) / 16 * 16 + 4;
+    const size_t lds = sizeof(unsigned) * ((size_t)TP * ld + (size_t)nt / 64 * LPX * 4);
+    const dim3 grid(tiles * (unsigned)p.batch), block((unsigned)nt);
+#define GNR_MAPS(RR) case RR: hipLaunchKernelGGL((quant_maps_kernel<T, LPX, RR>), grid, block, lds, st, p, tiles, ld); break
+    switch (R) { GNR_MAPS(1); GNR_MAPS(2); GNR_MAPS(3); GNR_MAPS(4); }
+#undef GNR_MAPS
+}
+// 32 pixels a tile.  Threads: the fewest that keep a row in 4 quads of channels each (64 maps of 258 x 4096 in fp32: 78 us with 256 threads,
+// 90 with 512), twice that where the tiles do not fill the card (one map: 6.9 against 5.7 us).
+template <typename T> static void quant_maps(const GnrRowsProblem& p, hipStream_t st) {
+    constexpr int LPX = 32 / Vec<T>::N;
     const int quads = (p.channels + 3) / 4;
     int nt = 64;
-    while (nt < 1024 && quads > nt / 8 * 4) nt *= 2;         // the fewest threads that keep the row in 4 quads each
-    const int G = nt / 8, R = quads >= 4 * G ? 4 : (quads + G - 1) / G;
-    const size_t lds = sizeof(unsigned) * ((size_t)TP * (G + 4) + (size_t)nt / 64 * TP);
-    const dim3 grid(tiles * (unsigned)p.batch), block((unsigned)nt);
-    switch (R) {
-        case 1: hipLaunchKernelGGL((quant_maps_kernel<T, 1>), grid, block, lds, st, p, tiles); break;
-        case 2: hipLaunchKernelGGL((quant_maps_kernel<T, 2>), grid, block, lds, st, p, tiles); break;
-        case 3: hipLaunchKernelGGL((quant_maps_kernel<T, 3>), grid, block, lds, st, p, tiles); break;
-        default: hipLaunchKernelGGL((quant_maps_kernel<T, 4>), grid, block, lds, st, p, tiles); break;
-    }
+    while (nt < 1024 && quads > nt / LPX * 4) nt *= 2;
+    if ((p.n_pix + 31) / 32 * p.batch < 512 && nt < 1024 && quads > nt / LPX) nt *= 2;
+    quant_maps_lpx<T, LPX>(p, nt, st);
 }
 
 template <typename T> static void quant_rows(const GnrRowsProblem& p, hipStream_t st) {
@@ -299,11 +316,13 @@ int launch_quantize(const GnrRowsProblem& p, hipStream_t st) {
     return e == hipSuccess ? 0 : fail("gnr_quantize_rows: launch failed: %s", hipGetErrorString(e));
 }
 
-template <typename T> static void read_maps(const GnrRowsProblem& p, hipStream_t st) {
-    constexpr int TP = 8 * Vec<T>::N;
+template <typename T, int LPX> static void read_maps_lpx(const GnrRowsProblem& p, hipStream_t st) {
+    constexpr int TP = LPX * Vec<T>::N;
     const unsigned tiles = (unsigned)((p.n_pix + TP - 1) / TP);
-    hipLaunchKernelGGL(read_maps_kernel<T>, dim3(tiles * (unsigned)p.batch), dim3(256), 0, st, p, tiles);
+    const int step = p.channels < 1920 ? p.channels : 1920, ld = (step + 63) / 64 * 16 + 4;
+    hipLaunchKernelGGL((read_maps_kernel<T, LPX>), dim3(tiles * (unsigned)p.batch), dim3(256), sizeof(unsigned) * TP * ld, st, p, tiles, ld, step);
 }
+template <typename T> static void read_maps(const GnrRowsProblem& p, hipStream_t st) { read_maps_lpx<T, sizeof(T) == 4 ? 8 : 4>(p, st); }
 
 }  // namespace gnr
 
