@@ -113,6 +113,12 @@ __device__ __forceinline__ SlotRef slot_of(const int64_t* slots, long n_slots, l
     return s < 0 ? SlotRef{0, 1} : (s >= n_slots ? SlotRef{0, 2} : SlotRef{s, 0});
 }
 
+// Workgroups go round robin over the 8 XCDs: block i works on tile (i % 8) (n / 8) + i / 8, so that one XCD walks neighbouring tiles
+__device__ __forceinline__ unsigned xcd_block(unsigned n) {
+    const unsigned per = n >> 3;
+    return blockIdx.x < per * 8 ? (blockIdx.x & 7) * per + (blockIdx.x >> 3) : blockIdx.x;
+}
+
 int check_rows(const GnrRowsProblem* p, const char* what);
 int launch_quantize(const GnrRowsProblem& p, hipStream_t st);        // defined in gnr_quant.hip; 0 == enqueued
 }  // namespace gnr

@@ -21,152 +21,366 @@ struct Int8Args {
     void* y;
     long P, N;                    // rows per batch entry, all rows
     int K, O, leaky;
+    const void* xf; long xf_pitch; // floating rows that the few-rows kernel quantises itself
+    int flat;                     // no slots, and every row of x a.x_pitch behind the one before (scales alike)
 };
 
-struct RowRef {
-    const int8_t* p;
-    float scale;
-};
-// row n of x: through the slot list if there is one
-__device__ __forceinline__ RowRef x_row(const Int8Args& a, long b, long pix) {
-    const SlotRef r = slot_of(a.slots, a.n_slots, b);
-    RowRef o;
-    o.p = a.x + r.slot * a.x_batch + (r.state ? 0 : pix) * a.x_pitch;
-    o.scale = r.state ? (r.state == 1 ? 0.0f : __uint_as_float(0x7fc00000u)) : a.xs[r.slot * a.xs_batch + pix];
-    return o;
+// Row r of x and its scale.  y [N][O]: r counts all rows; y [B][O][P]: r counts the pixels of entry b.
+__device__ __forceinline__ void x_at(const Int8Args& a, long& b, long& r, bool cf) {
+    if (!cf && !a.flat) {
+        b = (unsigned)r / (unsigned)a.P;
+        r = (unsigned)r - (unsigned)b * (unsigned)a.P;
+    }
+}
+__device__ __forceinline__ const int8_t* x_row(const Int8Args& a, long b, long r, bool cf) {
+    x_at(a, b, r, cf);
+    const SlotRef s = slot_of(a.slots, a.n_slots, b);
+    return a.x + s.slot * a.x_batch + r * a.x_pitch;          // an entry without a slot reads slot 0 and is multiplied by 0 or NaN
+}
+__device__ __forceinline__ float x_scale(const Int8Args& a, long b, long r, bool cf) {
+    x_at(a, b, r, cf);
+    const SlotRef s = slot_of(a.slots, a.n_slots, b);
+    return s.state ? (s.state == 1 ? 0.0f : __uint_as_float(0x7fc00000u)) : a.xs[s.slot * a.xs_batch + r];
 }
 
-__device__ __forceinline__ float leak(float v) { return v > 0.0f ? v : 0.2f * v; }
+__device__ __forceinline__ float leak(float v) { return fmaxf(v, 0.2f * v); }
 
 // ---------------------------------------------------------------------------------------------
-// the tiled product: WM x WN waves, each TM x TN tiles of 32 x 32
+// the tiled product: WM x WN waves, each TM x TN tiles of 32 x 32.
+//
+// K runs in stages of 64 bytes through a ring of NST LDS buffers that LDS-DMA fills (16 bytes a lane, no registers in between).  A stage
+// is two MFMA steps; while one is multiplied the fragments of the next are read, across the one barrier of a stage too:
+//     stage s + 1 has landed, barrier | step 1 of s, reading step 0 of s + 1 and requesting stage s + NST - 1 | step 0 of s + 1, reading step 1
+// (an odd number of steps leaves out step 0 of the FIRST stage: at the end, a step that may be left out costs a second set of accumulators).
+// The barrier of stage s stands behind every wave's reads of stage s - 1, whose buffer that request fills.  Reads and requests stand
+// between the MFMAs (in front of them they cost 1945 against 2124 TOP/s at 8192^3).
+// A 16-byte piece of tile row r sits at piece ^ ((r >> 1) & 3) of its 64 bytes (the swizzle is applied to the source address): the eight
+// lanes that read together hit eight different 16-byte columns.
+//
+// What a workgroup waits for (its first stage, its stores) is covered by the other workgroups of the CU, so registers and LDS are kept
+// low: accumulators in plain registers (launch bounds of two waves a SIMD), no more buffers than there are stages, an epilogue that turns
+// 4 KiB blocks a wave.  (Workgroups that walk several tiles and request the next one's stages under the epilogue were built: they need
+// twice the registers, and 262144 x 64 -> 32 took 9.2 us against 8.5, 458752 x 128 -> 256 64 against 56.)
 // ---------------------------------------------------------------------------------------------
-template <typename T, bool CF, int WM, int WN, int TM, int TN>
-__global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(const Int8Args a, unsigned tiles_m, unsigned tiles_n) {
-    constexpr int NW = WM * WN, NT = 64 * NW, BM = 32 * WM * TM, BN = 32 * WN * TN, BK = 64, PIECES = BK / 16;
-    constexpr int ROWS = BM + BN, LOADS = (ROWS * PIECES + NT - 1) / NT;                  // 16-byte pieces a thread stages per step
-    constexpr int EM = 32 * TM, ELD = EM + 4;                                  // epilogue: fp32 [32][EM + 4] per wave
-    constexpr int STAGE = ROWS * BK, EPI = NW * 32 * ELD * 4;
-    __shared__ __align__(16) char lds[STAGE > EPI ? STAGE : EPI];
-    __shared__ float sc[ROWS], bi[CF ? BN : BM];
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave % WM, wn = wave / WM;
-    const unsigned tm = blockIdx.x % tiles_m, rest = blockIdx.x / tiles_m, tn = rest % tiles_n;
-    const long b = rest / tiles_n;                                             // CF: batch entry; otherwise 0
-    const long m0 = (long)tm * BM, n0 = (long)tn * BN;
+__device__ __forceinline__ void dma16(const int8_t* p, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory");
+}
+template <int N> __device__ __forceinline__ void wait_vm() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N < 63 ? N : 63) : "memory");     // six bits; fewer than allowed is only stricter
+}
+__device__ __forceinline__ void tile_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+// the bytes at and behind `left` of a lane's 16 count as 0
+__device__ __forceinline__ i32x4 keep_bytes(i32x4 v, int left) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] &= left >= 4 * e + 4 ? -1 : (left <= 4 * e ? 0 : (1 << 8 * (left - 4 * e)) - 1);
+    return v;
+}
+
+template <int WM, int WN, int TM, int TN, int NST> struct TileShape {
+    static constexpr int NW = WM * WN, NT = 64 * NW, BM = 32 * WM * TM, BN = 32 * WN * TN, ROWS = BM + BN;
+    static constexpr int LOADS = (ROWS + 16 * NW - 1) / (16 * NW);             // requests of a wave per stage: 1 KiB = 16 rows each
+    static constexpr int STAGE = LOADS * NW * 1024, TURN = NW * 4096;
+};
+
+template <typename T, bool CF, int WM, int WN, int TM, int TN, int NST>
+__global__ __launch_bounds__(64 * WM * WN, 2) void int8_tile_kernel(const Int8Args a, unsigned tiles_m, unsigned tiles_n) {
+    typedef TileShape<WM, WN, TM, TN, NST> S;
+    constexpr int BM = S::BM, BN = S::BN, ROWS = S::ROWS, LOADS = S::LOADS, STAGE = S::STAGE, NT = S::NT, BK = 64;
+    constexpr int PAIR = sizeof(T) == 2 && TM % 2 == 0 ? 2 : 1;                // tiles of 32 x 32 that turn together
+    constexpr int EM = 32 * PAIR, RB = EM * (int)sizeof(T), PPR = RB / 16;     // their row of m: values, bytes, 16-byte pieces
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    __shared__ __attribute__((aligned(16))) float sc[ROWS], bi[CF ? BN : BM];
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
+    const int half = lane >> 5, sw = (lane >> 1) & 3, piece = (lane & 3) ^ ((lane >> 3) & 3);
     const long M = CF ? a.P : a.O, N = CF ? a.O : a.N;
+    const int K16 = (a.K + 15) & ~15, steps = (a.K + 31) / 32, odd = steps & 1, nst = (steps + odd) / 2;
+    const unsigned at = xcd_block(gridDim.x), tm = at % tiles_m, rest = at / tiles_m;
+    const long m0 = (long)tm * BM, n0 = (long)(rest % tiles_n) * BN, b = rest / tiles_n;       // b: CF, the batch entry; otherwise 0
 
-    // scales and bias of the tile's rows, and where each staged piece comes from
-    for (int i = tid; i < ROWS; i += NT) {
-        const bool is_m = i < BM;
-        const long r = is_m ? m0 + i : n0 + i - BM;
-        const bool is_x = is_m == CF;
-        float s = 0.0f, z = 0.0f;
-        if (r < (is_m ? M : N)) {
-            if (is_x) s = x_row(a, CF ? b : r / a.P, CF ? r : r % a.P).scale;
-            else { s = a.ws[r]; z = a.bias ? a.bias[r] : 0.0f; }
-        }
-        sc[i] = s;
-        if (!is_x) bi[is_m ? i : i - BM] = z;
-    }
     const int8_t* src[LOADS];
-    int dst[LOADS];
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
-        const int idx = tid + j * NT, i = idx / PIECES, piece = idx % PIECES;
+        const int i = (wave * LOADS + j) * 16 + (lane >> 2);
         const bool is_m = i < BM;
         const long lim = is_m ? M : N;
         long r = is_m ? m0 + i : n0 + i - BM;
-        r = i < ROWS && r < lim ? r : lim - 1;
-        src[j] = (is_m == CF ? x_row(a, CF ? b : r / a.P, CF ? r : r % a.P).p : a.w + r * a.w_pitch) + 16 * piece;
-        dst[j] = i * BK + 16 * (piece ^ ((i >> 1) & 3));                       // any 8 lanes of a fragment read: 8 different 16-byte slots
+        r = r < lim ? r : lim - 1;
+        src[j] = is_m == CF ? x_row(a, b, r, CF) : a.w + r * a.w_pitch;
     }
-    const int my_piece = tid % PIECES;
-    Vec<int> stage[LOADS];
-    auto load = [&](int k0) {
-        const int k = k0 + 16 * my_piece, left = a.K - k;                      // the bytes behind K of a row count as 0
+    constexpr int SCN = (ROWS + NT - 1) / NT;
+    float rs[SCN], rz[SCN];                                    // scales and bias of the tile's rows: requested first, needed last
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) {
-            Vec<int> v = {};
-            if (left > 0) {
-                __builtin_memcpy(&v, src[j] + k0, 16);
-                if (left < 16)
+    for (int j = 0; j < SCN; ++j) {
+        const int i = tid + j * NT;
+        const bool is_m = i < BM, is_x = is_m == CF;
+        const long r = is_m ? m0 + i : n0 + i - BM;
+        rs[j] = rz[j] = 0.0f;
+        if (i < ROWS && r < (is_m ? M : N)) {
+            if (is_x) rs[j] = x_scale(a, b, r, CF);
+            else { rs[j] = a.ws[r]; rz[j] = a.bias ? a.bias[r] : 0.0f; }
+        }
+    }
+    const unsigned lds0 = (unsigned)(size_t)&lds[0] + (unsigned)wave * LOADS * 1024u;
+    auto request_at = [&](int s, int& k, unsigned& d) {
+        k = s * BK - 32 * odd + 16 * piece;
+        k = k < 0 ? 0 : (k < K16 ? k : K16 - 16);              // inside the row always: the step before the first is not multiplied, what is
+                                                               // behind the last is masked
+        d = lds0 + (unsigned)(s % NST) * STAGE;
+    };
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        v.v[e] &= left >= 4 * e + 4 ? -1 : (left <= 4 * e ? 0 : (1 << 8 * (left - 4 * e)) - 1);
-            }
-            stage[j] = v;
+    for (int s = 0; s < NST - 1; ++s)
+        if (s < nst) {
+            int k; unsigned d;
+            request_at(s, k, d);
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) dma16(src[j] + k, d + j * 1024u);
+        }
+    i32x16 acc[TM][TN];
+    i32x4 f[2][TM + TN];
+    const int row_m = 32 * TM * wm + (lane & 31), row_n = BM + 32 * TN * wn + (lane & 31);
+    auto read = [&](int s, int step, int i) {
+        const char* base = lds + (s % NST) * STAGE + 16 * ((2 * step + half) ^ sw);
+        f[step][i] = *(const i32x4*)(base + (i < TM ? row_m + 32 * i : row_n + 32 * (i - TM)) * BK);
+    };
+    // the MFMAs of one step; behind each of them: a fragment of the step that follows (next_s < 0: none), and the requests of a stage
+    auto multiply = [&](int step, int next_s, int next_step, int req) {
+        constexpr int MF = TM * TN, RD = TM + TN;
+        int k; unsigned d;
+        request_at(req < 0 ? 0 : req, k, d);
+#pragma unroll
+        for (int t = 0; t < MF; ++t) {
+            acc[t / TN][t % TN] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[step][t / TN], f[step][TM + t % TN], acc[t / TN][t % TN], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < RD; ++i)
+                if (i * MF / RD == t && next_s >= 0) read(next_s, next_step, i);
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j)
+                if (j * MF / LOADS == t && req >= 0 && req < nst) dma16(src[j] + k, d + j * 1024u);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    i32x16 acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = i32x16{};
-
-    load(0);
-    for (int k0 = 0; k0 < a.K; k0 += BK) {
-        __syncthreads();
+    // Loads leave vmcnt in the order they were issued: what may stay outstanding is what was issued behind the stage that is needed
+    if (NST > 3 && nst > 2) wait_vm<2 * LOADS>();
+    else if (nst > 1) wait_vm<LOADS>();
+    else wait_vm<0>();
+    tile_barrier();
+    if (odd) {                                                 // the first stage has one step
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j)
-            if (tid + j * NT < ROWS * PIECES) __builtin_memcpy(lds + dst[j], &stage[j], 16);
-        __syncthreads();
-        if (k0 + BK < a.K) load(k0 + BK);
+        for (int i = 0; i < TM + TN; ++i) read(0, 1, i);
+    } else {
 #pragma unroll
-        for (int s = 0; s < BK / 32; ++s) {
-            if (k0 + 32 * s >= a.K) break;
-            const int piece = 2 * s + (lane >> 5);
-            i32x4 fm[TM], fn[TN];
+        for (int i = 0; i < TM + TN; ++i) read(0, 0, i);
+        multiply(0, 0, 1, -1);
+    }
+    for (int s = 0; s < nst - 1; ++s) {
+        if (NST > 3 && s + 2 < nst) wait_vm<LOADS>();
+        else wait_vm<0>();
+        tile_barrier();
+        multiply(1, s + 1, 0, s + NST - 1);
+        multiply(0, s + 1, 1, -1);
+    }
+    const int left = a.K - 32 * (steps - 1);                   // 1 .. 32 bytes of the last step exist
+    if (left < 32)
 #pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                const int r = 32 * (wm * TM + i) + (lane & 31);
-                fm[i] = *(const i32x4*)(lds + r * BK + 16 * (piece ^ ((r >> 1) & 3)));
-            }
+        for (int i = 0; i < TM + TN; ++i) f[1][i] = keep_bytes(f[1][i], left - 16 * half);
+    multiply(1, -1, 0, -1);
 #pragma unroll
-            for (int j = 0; j < TN; ++j) {
-                const int r = BM + 32 * (wn * TN + j) + (lane & 31);
-                fn[j] = *(const i32x4*)(lds + r * BK + 16 * (piece ^ ((r >> 1) & 3)));
-            }
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fm[i], fn[j], acc[i][j], 0, 0, 0);
+    for (int j = 0; j < SCN; ++j) {
+        const int i = tid + j * NT;
+        if (i < ROWS) {
+            sc[i] = rs[j];
+            if ((i < BM) != CF) bi[i < BM ? i : i - BM] = rz[j];
         }
     }
-    __syncthreads();
+    tile_barrier();                                            // every wave is done with the ring, too
 
-    // epilogue: scale, bias, activation in fp32; the wave's 32 x EM block turns in LDS so that stores run along m
-    float* e = (float*)lds + wave * 32 * ELD;
-    T* y = (T*)a.y + b * (long)a.O * a.P;
+    // epilogue: scale, bias, activation in fp32; 32 rows of n x EM values turn in LDS so that a row leaves as whole lines
+    char* turn = lds + wave * 4096;
+    const bool inside = m0 + BM <= M && n0 + BN <= N, lines = M * sizeof(T) % 128 == 0;
     const int mw = 32 * TM * wm;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-        const int nl = 32 * (wn * TN + j) + (lane & 31);
-        const float sn = sc[BM + nl], bn = CF ? bi[nl] : 0.0f;
+        const int nl = 32 * (wn * TN + j), nr = lane & 31;
+        const float sn = sc[BM + nl + nr], bn = CF ? bi[nl + nr] : 0.0f;
+        T* yn = (T*)a.y + b * (long)a.O * a.P + (n0 + nl) * M + m0 + mw;
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TM; ++i) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int ml = 32 * i + 8 * q + 4 * (lane >> 5);
-                fv4 v;
+                const int ml = 8 * q + 4 * half;
+                const fv4 sm = *(const fv4*)(sc + mw + 32 * i + ml), bm = CF ? fv4{bn, bn, bn, bn} : *(const fv4*)(bi + mw + 32 * i + ml);
+                typedef T t4 __attribute__((ext_vector_type(4)));
+                t4 o;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float sm = sc[mw + ml + r];
-                    // x_scale first: the larger of the two factors as a rule, the same order for both layouts
-                    const float t = (float)acc[i][j][4 * q + r] * (CF ? sm : sn) * (CF ? sn : sm) + (CF ? bn : bi[mw + ml + r]);
-                    v[r] = a.leaky ? leak(t) : t;
+                    // x_scale first, then w_scale: the same order for both layouts, hence the same bits
+                    float v = fmaf((float)acc[i][j][4 * q + r] * (CF ? sm[r] : sn), CF ? sn : sm[r], bm[r]);
+                    if (a.leaky) v = leak(v);
+                    o[r] = (T)v;
                 }
-                *(fv4*)(e + (lane & 31) * ELD + ml) = v;
+                const int at = 32 * (i % PAIR) + ml;
+                if constexpr (sizeof(T) == 4) *(t4*)(turn + nr * RB + 16 * ((at >> 2) ^ (nr & (PPR - 1)))) = o;
+                else *(t4*)(turn + nr * RB + 16 * ((at >> 3) ^ (nr & (PPR - 1))) + 2 * (at & 4)) = o;
             }
-        constexpr int V = Vec<T>::N, LPR = EM / V, RPI = 64 / LPR;             // lanes per row of m, rows per instruction
+            if (i % PAIR == PAIR - 1) {
 #pragma unroll
-        for (int it = 0; it < 32 / RPI; ++it) {
-            const int row = it * RPI + lane / LPR, m = (lane % LPR) * V;
-            const long n = n0 + 32 * (wn * TN + j) + row, mg = m0 + mw + m;
-            Vec<T> o;
+                for (int it = 0; it < 32 * PPR / 64; ++it) {
+                    const int row = it * (64 / PPR) + lane / PPR, pc = lane % PPR;
+                    Vec<T> o;
+                    __builtin_memcpy(&o, __builtin_assume_aligned(turn + row * RB + 16 * (pc ^ (row & (PPR - 1))), 16), 16);
+                    const int ml = 32 * (i - PAIR + 1) + Vec<T>::N * pc;
+                    T* p = yn + row * M + ml;
+                    if (inside && lines) store_part<true>(p, o, Vec<T>::N);
+                    else if (inside) store_part(p, o, Vec<T>::N);
+                    else if (n0 + nl + row < N && m0 + mw + ml < M) {
+                        const long left = M - m0 - mw - ml;
+                        store_part(p, o, left < Vec<T>::N ? (int)left : Vec<T>::N);
+                    }
+                }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// few rows (at most 16 TT): the time to read the weights.  A workgroup owns 16 outputs; its four waves share K in steps of 64 bytes
+// (v_mfma_i32_16x16x64_i8: lane l holds row l % 16, bytes 16 (l / 16) ..) and keep eight steps of weights in flight, fragments
+// straight from memory; the four partial sums are whole numbers and meet in LDS.  Floating x is quantised by every workgroup
+// for itself (TT == 1): one launch instead of two.
+// ---------------------------------------------------------------------------------------------
+constexpr int FEW_MAX = 64, FEW_FUSED = 16, FEW_FUSED_K = 4096;
+
+template <typename X, typename T, bool CF, int TT>
+__global__ __launch_bounds__(256) void int8_few_kernel(const Int8Args a) {
+    constexpr bool FLOAT = !__is_same(X, int8_t);
+    constexpr int U = TT == 1 ? 8 : 4;                         // steps in flight
+    extern __shared__ __attribute__((aligned(16))) char lds[];                 // FLOAT: rows of x, [16][ld]; then the partial sums
+    __shared__ float xsc[16 * TT];
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, kq = 16 * (lane >> 4);
+    const int N = (int)a.N, K = a.K, K16 = (K + 15) & ~15, nst = (K + 63) / 64, o0 = (int)blockIdx.x * 16;
+    const int ld = nst * 64 + 16;
+    const int o = o0 + col < a.O ? o0 + col : a.O - 1;
+    const int8_t* wp = a.w + (long)o * a.w_pitch;
+    const int8_t* xp[TT];
+    if constexpr (!FLOAT) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) o.v[v] = (T)e[row * ELD + m + v];
-            const long left = M - mg;
-            if (n < N && left > 0) store_part(y + n * M + mg, o, left < V ? (int)left : V);
+        for (int t = 0; t < TT; ++t) {
+            const int n = 16 * t + col < N ? 16 * t + col : N - 1;
+            xp[t] = x_row(a, 0, n, false);
+        }
+        if (tid < 16 * TT) xsc[tid] = x_scale(a, 0, tid < N ? tid : N - 1, false);
+    }
+    i32x4 w[U], x[U][TT];
+    auto load = [&](int s0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int s = s0 + 4 * u;
+            if (s < nst) {
+                const int k = s * 64 + kq < K16 ? s * 64 + kq : K16 - 16;      // never behind a row; masked below
+                w[u] = *(const i32x4*)(wp + k);
+                if constexpr (!FLOAT)
+#pragma unroll
+                    for (int t = 0; t < TT; ++t) x[u][t] = *(const i32x4*)(xp[t] + k);
+            }
+        }
+    };
+    load(wave);                                                // under the quantisation
+    if constexpr (FLOAT) {
+        constexpr int V = Vec<X>::N, J = FEW_FUSED_K / 2 / (64 * 4);           // 8 pieces a lane: 2048 values in fp32, 4096 in 16 bits
+        const X* xb = (const X*)a.xf;
+        for (int n = wave; n < N; n += 4) {
+            const X* row = xb + (long)n * a.xf_pitch;
+            Raw16 r[J];
+            unsigned m[4] = {};
+            auto get = [&](int j0) {
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    const int c = ((j0 + j) * 64 + lane) * V;
+                    r[j] = c < K ? load_raw(row + c, K - c) : Raw16{};
+                }
+            };
+            const int pieces = (K + 64 * V - 1) / (64 * V);
+            for (int j0 = 0; j0 < pieces; j0 += J) {
+                get(j0);
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) m[i] = max_bits<X>(m[i], r[j].w[i]);
+            }
+            m[0] = max_bits<X>(max_bits<X>(m[0], m[1]), max_bits<X>(m[2], m[3]));
+#pragma unroll
+            for (int i = 1; i < 64; i <<= 1) m[0] = max_bits<X>(m[0], (unsigned)__shfl_xor((int)m[0], i));
+            if constexpr (sizeof(X) == 2) m[0] = max_bits<X>(m[0], m[0] >> 16);
+            float s, per;
+            row_scale(__float_as_uint(raw_value<X>(m, 0)), s, per);
+            if (lane == 0) xsc[n] = s;
+            for (int j0 = 0; j0 < pieces; j0 += J) {
+                if (pieces > J) get(j0);
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    const int c = ((j0 + j) * 64 + lane) * V;                  // bytes behind K become 0: load_raw filled up with 0
+                    if (c < nst * 64) {
+                        unsigned q[V / 4];
+#pragma unroll
+                        for (int i = 0; i < V / 4; ++i)
+                            q[i] = pack4(row_step(raw_value<X>(r[j].w, 4 * i), per), row_step(raw_value<X>(r[j].w, 4 * i + 1), per),
+                                         row_step(raw_value<X>(r[j].w, 4 * i + 2), per), row_step(raw_value<X>(r[j].w, 4 * i + 3), per));
+                        __builtin_memcpy(__builtin_assume_aligned(lds + n * ld + c, V), q, V);
+                    }
+                }
+            }
+        }
+    }
+    i32x4 acc[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[t] = i32x4{};
+    if constexpr (FLOAT) __syncthreads();
+    for (int s0 = wave; s0 < nst; s0 += 4 * U) {
+        if (s0 != wave) load(s0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int s = s0 + 4 * u;
+            if (s >= nst) break;
+            const int left = K - s * 64 - kq;
+            if (K - s * 64 < 64) w[u] = keep_bytes(w[u], left);
+#pragma unroll
+            for (int t = 0; t < TT; ++t) {
+                if constexpr (FLOAT) x[u][t] = *(const i32x4*)(lds + (col < N ? col : 0) * ld + s * 64 + kq);
+                else if (K - s * 64 < 64) x[u][t] = keep_bytes(x[u][t], left);
+                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u], x[u][t], acc[t], 0, 0, 0);
+            }
+        }
+    }
+    __syncthreads();                                           // the rows in LDS have been read
+    i32x4* part = (i32x4*)lds;                                 // [wave][TT][64]
+#pragma unroll
+    for (int t = 0; t < TT; ++t) part[(wave * TT + t) * 64 + lane] = acc[t];
+    __syncthreads();
+    for (int t = wave; t < TT; t += 4) {
+        i32x4 sum = part[t * 64 + lane];
+#pragma unroll
+        for (int v = 1; v < 4; ++v) sum += part[(v * TT + t) * 64 + lane];
+        const int n = 16 * t + col;
+        if (n >= N) continue;
+        const float sx = xsc[n];
+        const int P = (int)a.P;
+        T* y = CF ? (T*)a.y + (long)(n / P) * a.O * P + n % P : (T*)a.y + (long)n * a.O;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int oo = o0 + 4 * (lane >> 4) + r;
+            if (oo < a.O) {
+                float v = fmaf((float)sum[r] * sx, a.ws[oo], a.bias ? a.bias[oo] : 0.0f);
+                if (a.leaky) v = leak(v);
+                y[CF ? (long)oo * P : (long)oo] = (T)v;
+            }
         }
     }
 }
@@ -203,38 +417,69 @@ static int check_int8(const GnrInt8Problem* p) {
     return 0;
 }
 
+// floating rows that the few-rows kernel takes as they are
+static bool int8_fused(const GnrInt8Problem* p) {
+    return p->x_type != GNR_I8 && !p->x_channels_first && !p->y_channels_first && p->batch == 1 && p->n_pix <= FEW_FUSED && p->k <= FEW_FUSED_K;
+}
+
 struct Int8Ws {
     size_t q_pitch, q_bytes, bytes;
 };
 static Int8Ws int8_ws(const GnrInt8Problem* p) {                     // floating x: its rows and their scales
     Int8Ws w{};
-    if (p->x_type == GNR_I8) return w;
+    if (p->x_type == GNR_I8 || int8_fused(p)) return w;
     const size_t n = (size_t)p->batch * (size_t)p->n_pix;
-    w.q_pitch = ((size_t)p->k + 15) & ~(size_t)15;
+    w.q_pitch = ((size_t)p->k + 63) & ~(size_t)63;                   // a stage of a row never crosses a line: 28672 x 516 -> 1032 41 -> 38 us
     w.q_bytes = (n * w.q_pitch + 255) & ~(size_t)255;
     w.bytes = w.q_bytes + ((n * sizeof(float) + 255) & ~(size_t)255);
     return w;
 }
 
-template <typename T, bool CF, int WM, int WN, int TM, int TN> static int launch_tile(const Int8Args& a, long batch, hipStream_t st) {
-    constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN;
+template <typename T, bool CF, int WM, int WN, int TM, int TN, int NST = 4> static int launch_tile(const Int8Args& a, long batch, hipStream_t st) {
+    typedef TileShape<WM, WN, TM, TN, NST> S;
     const long M = CF ? a.P : a.O, N = CF ? a.O : a.N;
-    const long tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN, blocks = tm * tn * (CF ? batch : 1);
-    if (blocks >= (1L << 31)) return fail("gnr_int8_linear: %ld tiles exceed one launch", blocks);
-    hipLaunchKernelGGL((int8_tile_kernel<T, CF, WM, WN, TM, TN>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, st, a, (unsigned)tm, (unsigned)tn);
+    const long tm = (M + S::BM - 1) / S::BM, tn = (N + S::BN - 1) / S::BN, tiles = tm * tn * (CF ? batch : 1);
+    if (tiles >= (1L << 31)) return fail("gnr_int8_linear: %ld tiles exceed one launch", tiles);
+    const int stages = (a.K + 63) / 64 < NST ? (a.K + 63) / 64 : NST, ring = stages * S::STAGE;
+    hipLaunchKernelGGL((int8_tile_kernel<T, CF, WM, WN, TM, TN, NST>), dim3((unsigned)tiles), dim3(S::NT), ring > S::TURN ? ring : S::TURN, st, a,
+                       (unsigned)tm, (unsigned)tn);
     return 0;
 }
 
-template <typename T> static int launch_int8(const Int8Args& a, long batch, bool cf, hipStream_t st) {
-    if (cf) {
-        if (a.O <= 32) return launch_tile<T, true, 4, 1, 2, 1>(a, batch, st);
-        if (a.O <= 64) return launch_tile<T, true, 4, 1, 2, 2>(a, batch, st);
-        return launch_tile<T, true, 2, 2, 2, 2>(a, batch, st);
-    }
-    if (a.O <= 64) return launch_tile<T, false, 1, 4, 2, 2>(a, batch, st);
-    return launch_tile<T, false, 2, 2, 2, 2>(a, batch, st);
+template <typename X, typename T, bool CF, int TT> static void launch_few(const Int8Args& a, hipStream_t st) {
+    const int rows = 16 * (((a.K + 63) / 64) * 64 + 16), part = 4 * TT * 64 * 16;
+    hipLaunchKernelGGL((int8_few_kernel<X, T, CF, TT>), dim3((unsigned)((a.O + 15) / 16)), dim3(256),
+                       !__is_same(X, int8_t) && rows > part ? rows : part, st, a);
 }
 
+// Which kernel.  Figures: us on one card, bf16 y unless stated, rows x K -> O.
+//   at most 64 rows       the few-rows kernel (1 x 2048 -> 4096: 64 x 64 tiles 10)
+//   O <= 32, 64           tiles as narrow as the layer (262144 x 64 -> 32, fp32 maps: 8.0 against 9.0 with 64 rows a wave)
+//   256 x 256 tiles       where they fill the card and K is long: 16384 x 2048 -> 4096 150 against 196 with 128 x 128, but
+//                         28672 x 516 -> 1032 47 against 41: there it is y that takes the time
+//   128 x 128, 64 x 64    by whether the larger fill the card (4096 x 258 -> 516, fp32: 64 x 64 6.2, 128 x 128 8.3)
+template <typename T, bool CF> static int launch_int8(const Int8Args& a, long batch, hipStream_t st) {
+    if (a.N <= FEW_MAX) {
+        if (a.N <= 16) launch_few<int8_t, T, CF, 1>(a, st);
+        else if (a.N <= 32) launch_few<int8_t, T, CF, 2>(a, st);
+        else launch_few<int8_t, T, CF, 4>(a, st);
+        return 0;
+    }
+    // m: outputs (y [N][O]) or pixels (y [B][O][P])
+    const long M = CF ? a.P : a.O, N = CF ? a.O : a.N, B = CF ? batch : 1;
+    const long t256 = ((M + 255) / 256) * ((N + 255) / 256) * B, t128 = ((M + 127) / 128) * ((N + 127) / 128) * B;
+    constexpr int WM = CF ? 4 : 1, WN = CF ? 1 : 4;
+    if (a.O <= 32) return launch_tile<T, CF, WM, WN, 1, 1, 3>(a, batch, st);
+    if (a.O <= 64) return launch_tile<T, CF, WM, WN, CF ? 1 : 2, CF ? 2 : 1, 3>(a, batch, st);
+    if (t256 >= 256 && a.K >= 1024) return launch_tile<T, CF, 2, 4, 4, 2, 4>(a, batch, st);
+    if (t128 >= 256) return launch_tile<T, CF, 2, 2, 2, 2, 3>(a, batch, st);
+    return launch_tile<T, CF, 2, 2, 1, 1, 4>(a, batch, st);
+}
+template <typename X> static void launch_fused(const Int8Args& a, int y_type, hipStream_t st) {
+    if (y_type == GNR_F32) launch_few<X, float, false, 1>(a, st);
+    else if (y_type == GNR_BF16) launch_few<X, __bf16, false, 1>(a, st);
+    else launch_few<X, _Float16, false, 1>(a, st);
+}
 }  // namespace gnr
 
 using namespace gnr;
@@ -257,6 +502,13 @@ int gnr_int8_linear(const GnrInt8Problem* p, void* workspace, size_t ws_bytes, v
     if (p->x_type == GNR_I8) {
         a.x = (const int8_t*)p->x; a.x_batch = p->x_batch; a.x_pitch = p->x_stride; a.xs = p->x_scale; a.xs_batch = p->x_scale_batch;
         a.slots = p->slots; a.n_slots = p->n_slots;
+    } else if (int8_fused(p)) {
+        a.xf = p->x; a.xf_pitch = p->x_stride;
+        if (p->x_type == GNR_F32) launch_fused<float>(a, p->y_type, st);
+        else if (p->x_type == GNR_BF16) launch_fused<__bf16>(a, p->y_type, st);
+        else launch_fused<_Float16>(a, p->y_type, st);
+        const hipError_t e = hipGetLastError();
+        return e == hipSuccess ? 0 : fail("gnr_int8_linear: launch failed: %s", hipGetErrorString(e));
     } else {
         const Int8Ws w = int8_ws(p);
         if (!workspace || ws_bytes < w.bytes) return fail("gnr_int8_linear: workspace too small (%zu < %zu bytes)", ws_bytes, w.bytes);
@@ -270,9 +522,11 @@ int gnr_int8_linear(const GnrInt8Problem* p, void* workspace, size_t ws_bytes, v
         a.x = r.q; a.x_batch = r.q_batch; a.x_pitch = r.q_pitch; a.xs = r.scale; a.xs_batch = p->n_pix;
     }
     int rc;
-    if (p->y_type == GNR_F32) rc = launch_int8<float>(a, p->batch, p->y_channels_first != 0, st);
-    else if (p->y_type == GNR_BF16) rc = launch_int8<__bf16>(a, p->batch, p->y_channels_first != 0, st);
-    else rc = launch_int8<_Float16>(a, p->batch, p->y_channels_first != 0, st);
+    const bool cf = p->y_channels_first != 0;
+    a.flat = !a.slots && (p->batch == 1 || (a.x_batch == a.P * a.x_pitch && a.xs_batch == a.P));
+    if (p->y_type == GNR_F32) rc = cf ? launch_int8<float, true>(a, p->batch, st) : launch_int8<float, false>(a, p->batch, st);
+    else if (p->y_type == GNR_BF16) rc = cf ? launch_int8<__bf16, true>(a, p->batch, st) : launch_int8<__bf16, false>(a, p->batch, st);
+    else rc = cf ? launch_int8<_Float16, true>(a, p->batch, st) : launch_int8<_Float16, false>(a, p->batch, st);
     if (rc) return 1;
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail("gnr_int8_linear: launch failed: %s", hipGetErrorString(e));

@@ -8,11 +8,6 @@
 
 namespace gnr {
 
-// Workgroups go round robin over the 8 XCDs: block i works on tile (i % 8) (n / 8) + i / 8, so that one XCD walks neighbouring tiles
-__device__ __forceinline__ unsigned xcd_block(unsigned n) {
-    const unsigned per = n >> 3;
-    return blockIdx.x < per * 8 ? (blockIdx.x & 7) * per + (blockIdx.x >> 3) : blockIdx.x;
-}
 __device__ __forceinline__ long tile_start(unsigned i, int tp, long n) {
     const long p = (long)i * tp;
     return p + tp <= n || n < tp ? p : n - tp;
