@@ -97,6 +97,13 @@ class GnrInt8Problem(_Sized):
                 ("w_scale", _p), ("bias", _p), ("y", _p)]
 
 
+class GnrUpsampleInt8(_Sized):
+    _fields_ = [("struct_size", C.c_uint32), ("reserved", C.c_uint32)] + [
+        (n + k, t * UP_MAX) for n in ("up1", "up2", "feat") for k, t in (("_w", _p), ("_pitch", C.c_int64), ("_s", _p))] + [
+        ("x_q", _p), ("x_batch", C.c_int64), ("x_pitch", C.c_int64), ("x_scale", _p), ("x_scale_batch", C.c_int64), ("slots", _p),
+        ("n_slots", C.c_int64)]
+
+
 class GnrInputGrads(C.Structure):
     _fields_ = [("R", _p), ("T", _p), ("shape_code", _p), ("gaze", _p), ("appea_code", _p), ("ray_bias", _p * 2)]
 
@@ -104,11 +111,12 @@ class GnrInputGrads(C.Structure):
 EXPORTS = ("gnr_abi_version", "gnr_build_info", "gnr_set_conv16_tile", "gnr_sizeof", "gnr_workspace_bytes", "gnr_fwd", "gnr_fwd_bf16x3", "gnr_bwd", "gnr_bwd_bf16x3", "gnr_resample",
            "gnr_sample_zvals", "gnr_set_kernel_timing", "gnr_set_aux_timing", "gnr_set_stage_timing", "gnr_set_clock_probe", "gnr_merge_scratch_bytes",
            "gnr_merge_fwd", "gnr_merge_bwd", "gnr_upsample_workspace_bytes", "gnr_upsample_fwd", "gnr_upsample_bwd",
-           "gnr_quantize_rows", "gnr_read_rows", "gnr_int8_linear_workspace_bytes", "gnr_int8_linear", "gnr_last_error")
+           "gnr_quantize_rows", "gnr_read_rows", "gnr_int8_linear_workspace_bytes", "gnr_int8_linear", "gnr_upsample_int8_workspace_bytes",
+           "gnr_upsample_int8_fwd", "gnr_last_error")
 
 # order == the GNR_SIZEOF_* ids of include/gnr.h
 STRUCTS = (GnrProblem, GnrWeights, GnrOutputs, GnrOutputGrads, GnrInputGrads, GnrMergeProblem, GnrUpsampleProblem,
-           GnrUpsampleWeights, GnrRowsProblem, GnrInt8Problem)
+           GnrUpsampleWeights, GnrRowsProblem, GnrInt8Problem, GnrUpsampleInt8)
 
 _lib = None
 
@@ -218,6 +226,11 @@ def load():
     lib.gnr_int8_linear_workspace_bytes.argtypes = [C.POINTER(GnrInt8Problem)]
     lib.gnr_int8_linear.restype = C.c_int
     lib.gnr_int8_linear.argtypes = [C.POINTER(GnrInt8Problem), _p, C.c_size_t, _p]
+    lib.gnr_upsample_int8_workspace_bytes.restype = C.c_size_t
+    lib.gnr_upsample_int8_workspace_bytes.argtypes = [C.POINTER(GnrUpsampleProblem), C.POINTER(GnrUpsampleInt8)]
+    lib.gnr_upsample_int8_fwd.restype = C.c_int
+    lib.gnr_upsample_int8_fwd.argtypes = [C.POINTER(GnrUpsampleProblem), C.POINTER(GnrUpsampleWeights), C.POINTER(GnrUpsampleInt8), _p, _p,
+                                          C.c_size_t, _p]
     lib.gnr_sizeof.restype = C.c_size_t
     lib.gnr_sizeof.argtypes = [C.c_int]
     for which, cls in enumerate(STRUCTS):

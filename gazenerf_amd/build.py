@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "build")
 LIB = os.path.join(HERE, "libgnr.so")
-SOURCES = ["gnr_api.hip", "gnr_prep.hip", "gnr_fwd16.hip", "gnr_bwd.hip", "gnr_bwd16.hip", "gnr_wgrad.hip", "gnr_wgrad16.hip", "gnr_merge.hip", "gnr_vd.hip", "gnr_fwd3.hip", "gnr_bwd3.hip", "gnr_conv16.hip", "gnr_upsample.hip", "gnr_quant.hip", "gnr_int8.hip"]
+SOURCES = ["gnr_api.hip", "gnr_prep.hip", "gnr_fwd16.hip", "gnr_bwd.hip", "gnr_bwd16.hip", "gnr_wgrad.hip", "gnr_wgrad16.hip", "gnr_merge.hip", "gnr_vd.hip", "gnr_fwd3.hip", "gnr_bwd3.hip", "gnr_conv16.hip", "gnr_upsample.hip", "gnr_quant.hip", "gnr_int8.hip", "gnr_upsample8.hip"]
 HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith(".h")) + [os.path.join("..", "..", "include", "gnr.h")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function"]
@@ -29,7 +29,8 @@ STAMP = os.path.join(OBJ, "build_info.txt")
 # per-file extras.  gnr_wgrad.hip: the SLP vectoriser packs the scalar rider adds that sit between the MFMAs into
 # v_pk_* with register shuffles around them -- each extra VALU instruction there costs matrix-pipe cycles.
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]     # scalar fp32 only: some packed forms have given wrong results
-EXTRA_FLAGS = {"gnr_wgrad.hip": ["-fno-slp-vectorize"], "gnr_quant.hip": NO_PACKED_FP32, "gnr_int8.hip": NO_PACKED_FP32}
+EXTRA_FLAGS = {"gnr_wgrad.hip": ["-fno-slp-vectorize"], "gnr_quant.hip": NO_PACKED_FP32, "gnr_int8.hip": NO_PACKED_FP32,
+               "gnr_upsample8.hip": NO_PACKED_FP32}
 
 
 def _stale(target, deps):

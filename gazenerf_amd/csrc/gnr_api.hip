@@ -264,6 +264,7 @@ size_t gnr_sizeof(int which) {
         case GNR_SIZEOF_UPSAMPLE_WEIGHTS: return sizeof(GnrUpsampleWeights);
         case GNR_SIZEOF_ROWS_PROBLEM: return sizeof(GnrRowsProblem);
         case GNR_SIZEOF_INT8_PROBLEM: return sizeof(GnrInt8Problem);
+        case GNR_SIZEOF_UPSAMPLE_INT8: return sizeof(GnrUpsampleInt8);
         default: return 0;
     }
 }

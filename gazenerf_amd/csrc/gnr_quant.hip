@@ -121,7 +121,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const GnrRowsProblem p,
     const int lane = (int)threadIdx.x % L;
     const long n = (long)blockIdx.x * (256 / L) + (int)threadIdx.x / L;
     const bool ok = n < total;
-    const long b = ok ? n / p.n_pix : 0, pix = ok ? n % p.n_pix : 0;
+    const unsigned b = ok ? (unsigned)n / (unsigned)p.n_pix : 0, pix = ok ? (unsigned)n - b * (unsigned)p.n_pix : 0;     // rows: at most 2^31
     const T* x = (const T*)p.x + b * p.x_batch + pix * p.x_stride;
     int8_t* q = p.q + b * p.q_batch + pix * p.q_pitch;
     const int C = p.channels, step = L * J * V, n_chunk = (C + step - 1) / step;

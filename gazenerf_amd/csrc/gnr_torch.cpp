@@ -281,7 +281,7 @@ void check_on(const Tensor& t, const char* name, at::ScalarType type, int64_t di
 void check_cuda(const Tensor& t, const char* name) {
     TORCH_CHECK(t.defined() && t.is_cuda(), name, " must live on a CUDA/ROCm device (the 8-bit operators have no CPU path)");
 }
-int64_t row_pitch(int64_t k) { return (k + 15) / 16 * 16; }
+int64_t row_pitch(int64_t k) { return (k + 63) / 64 * 64; }
 Tensor empty_rows(int64_t b, int64_t n, int64_t k, const c10::Device& dev) {
     Tensor t = at::empty({b, n, row_pitch(k)}, at::TensorOptions().dtype(at::kChar).device(dev));
     return t.slice(2, 0, k);
@@ -313,7 +313,7 @@ Tensor rows3(const Tensor& t) {
 int64_t stride_or(const Tensor& t, int64_t d, int64_t other) { return t.size(d) > 1 ? t.stride(d) : other; }
 // 8-bit rows [b, n, K] as a product reads them: on 16-byte boundaries, readable to the next multiple of 16
 Tensor pitched(const Tensor& q) {
-    const int64_t b = q.size(0), n = q.size(1), k = q.size(2), k16 = row_pitch(k);
+    const int64_t b = q.size(0), n = q.size(1), k = q.size(2), k16 = (k + 15) / 16 * 16;
     bool ok = (k == 1 || q.stride(2) == 1) && (n <= 1 || (q.stride(1) % 16 == 0 && q.stride(1) >= k16)) &&
               (b <= 1 || q.stride(0) % 16 == 0) && (uintptr_t)q.data_ptr() % 16 == 0;
     if (ok && q.numel() != 0) {

@@ -31,6 +31,7 @@
 #include "gnr_canary.h"
 #include "gnr_conv16.h"
 #include "gnr_device.h"
+#include "gnr_upsample.h"
 #include "gnr_wgrad.h"
 
 namespace gnr {
@@ -736,11 +737,7 @@ __global__ __launch_bounds__(256) void unshuffle_dres_kernel(const float* __rest
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
-struct UpDims {
-    int n_blocks, ch[UP_MAX + 1], side[UP_MAX + 1];
-};
-
-static int up_dims(const GnrUpsampleProblem* p, UpDims* d) {
+int up_dims(const GnrUpsampleProblem* p, UpDims* d) {
     if (!p) return fail("gnr_upsample: problem is NULL");
     if (p->struct_size != sizeof(GnrUpsampleProblem))
         return fail("gnr_upsample: GnrUpsampleProblem.struct_size is %u but this libgnr.so (ABI %d) has sizeof = %zu: the caller "
@@ -979,7 +976,7 @@ static void launch_rgb_conv(const float* net, int C, long P, int batch, const fl
 }
 
 // out <- blur(bilinear2x(in)) for 3-channel images at side S -> 2S, one kernel (round 4; two before)
-static void up_rgb(const float* in, float* out, int batch, int S, hipStream_t st) {       // in != out
+void up_rgb(const float* in, float* out, int batch, int S, hipStream_t st) {       // in != out
     const long planes = (long)batch * 3;
     hipLaunchKernelGGL(bilinear_blur_kernel, dim3(blocks_for(planes * 4L * S * S / 4)), dim3(256), 0, st, in, out, planes, S, S);
 }

@@ -193,12 +193,32 @@ class GazeNeRFNetAMD(HotPathRenderer):
     (gaze_nerf.py:318-331) plus ``t_rand`` to pin the train-mode jitter, and returns
     ``{"coarse_dict": {"merge_img_face", "merge_img_eyes", "merge_img", "bg_img"}}`` like the reference."""
 
-    def __init__(self, featmap_size: int = 64, pred_img_size: int = 512, bg_type: str = "white", **kw):
+    def __init__(self, featmap_size: int = 64, pred_img_size: int = 512, bg_type: str = "white", renderer_precision: str = "fp32", **kw):
         super().__init__(**kw)
         from .upsample import NeuralRendererAMD
         self.featmap_size, self.pred_img_size = featmap_size, pred_img_size
         self.neural_render = NeuralRendererAMD(bg_type=bg_type, feat_nc=self.featmap_nc, out_dim=3, final_actvn=True,
-                                               min_feat=32, featmap_size=featmap_size, img_size=pred_img_size)
+                                               min_feat=32, featmap_size=featmap_size, img_size=pred_img_size,
+                                               precision=renderer_precision)
+
+    @torch.no_grad()
+    def cache_views(self, cache, slots, batch_xy, shape_code, appea_code, gaze_code, batch_Rmats, batch_Tvecs, batch_inv_inmats):
+        """Renders the views' merged feature maps ("test" mode) into ``slots`` of a ``FeatureMapCache`` of 8-bit rows: what a viewer or a
+        sweep shows again and again (the reference's render loops, utils/render_utils.py:101-221) is rendered once."""
+        from .merge import merge_featmaps
+        out = HotPathRenderer.forward(self, batch_xy, batch_Rmats, batch_Tvecs, batch_inv_inmats, shape_code, appea_code, gaze_code)
+        S, C = self.featmap_size, self.featmap_nc
+        if batch_xy.shape[2] != S * S:
+            raise ValueError("batch_xy must cover the %dx%d feature map" % (S, S))
+        bg = self.neural_render.get_bg_featmap()
+        merged = merge_featmaps(out["feat_face"], out["bg_alpha_face"], out["feat_eyes"], out["bg_alpha_eyes"], bg.reshape(1, C, S * S),
+                                gaze_code.reshape(-1, 2))[2]
+        cache.write(slots, merged)
+
+    @torch.no_grad()
+    def render_views(self, cache, slots):
+        """Images [B, 3, ..] of cached views (``merge_img`` of ``forward`` in 8 bits): the upsampler alone, from the cached rows."""
+        return self.neural_render.render_cached(cache, slots)
 
     def forward(self, mode, batch_xy, batch_uv, bg_code, shape_code, appea_code, gaze_code, batch_Rmats, batch_Tvecs,
                 batch_inv_inmats, dist_expr=False, t_rand: Optional[torch.Tensor] = None, **kwargs):

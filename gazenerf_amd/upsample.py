@@ -258,8 +258,15 @@ class NeuralRendererAMD(nn.Module):
     shapes and initialisation; ``forward`` runs on the HIP kernels)."""
 
     def __init__(self, bg_type="white", feat_nc=258, out_dim=3, final_actvn=True, min_feat=32, featmap_size=64,
-                 img_size=512, graph_inference=True, **kwargs):
+                 img_size=512, graph_inference=True, precision="fp32", **kwargs):
         super().__init__()
+        from .upsample8 import GraphedUpsample8, Int8Weights
+        # precision="int8": inference in 8 bits (gazenerf_amd.upsample8); calls that need gradients are refused
+        if precision not in ("fp32", "int8"):
+            raise ValueError("precision must be 'fp32' or 'int8'")
+        self.precision = precision
+        self._int8_weights = Int8Weights()
+        self._graphed8 = GraphedUpsample8(self._int8_weights)
         # graph_inference: under torch.no_grad() the forward is replayed from a HIP graph (GraphedUpsample) -- the
         # reference's render loops call the network one image at a time, where launch gaps were a fifth of the call
         self.graph_inference = bool(graph_inference)
@@ -284,7 +291,25 @@ class NeuralRendererAMD(nn.Module):
     def get_bg_featmap(self):
         return self.bg_featmap
 
+    def _render_int8(self, x=None, cache=None, slots=None):
+        from .upsample8 import neural_render_int8
+        params = {k: v for k, v in self.named_parameters() if k != "bg_featmap"}
+        dev = x if x is not None else cache.q
+        if self.graph_inference and not torch.is_grad_enabled() and dev.is_cuda and not torch.cuda.is_current_stream_capturing():
+            return self._graphed8(params, self.n_blocks, self.min_feat, self.final_actvn, x, cache, slots)
+        return neural_render_int8(x, params, self.n_blocks, self.min_feat, self.final_actvn, self._int8_weights, cache, slots)
+
+    def render_cached(self, cache, slots):
+        """Images [B, 3, ..] of the feature maps in ``slots`` of a ``FeatureMapCache`` (an int, a sequence or an int64 tensor on its device), in
+        8 bits whatever ``precision`` says: the first convolution reads the cached rows.  Call under ``torch.no_grad()``."""
+        if cache.q.shape[2] != self.n_feat or cache.q.shape[1] != self.featmap_size ** 2:
+            raise ValueError("the cache holds maps of %d channels x %d pixels, the renderer takes %d x %d" % (
+                cache.q.shape[2], cache.q.shape[1], self.n_feat, self.featmap_size ** 2))
+        return self._render_int8(None, cache, cache.slots(slots))
+
     def forward(self, x):
+        if self.precision == "int8":
+            return self._render_int8(x)
         params = {k: v for k, v in self.named_parameters() if k != "bg_featmap"}
         if (self.graph_inference and not torch.is_grad_enabled() and x.is_cuda and x.dtype == torch.float32 and x.dim() == 4
                 and not torch.cuda.is_current_stream_capturing()):
@@ -293,4 +318,14 @@ class NeuralRendererAMD(nn.Module):
 
     def _apply(self, fn, *args, **kw):          # .to() / .cuda() / .half(): parameters move, captured graphs are stale
         self._graphed.clear()
+        self._graphed8.clear()
+        self._int8_weights.clear()
         return super()._apply(fn, *args, **kw)
+
+    def train(self, mode: bool = True):         # the quantised weights would miss an in-place write through ``.data``
+        self._int8_weights.seen = None
+        return super().train(mode)
+
+    def load_state_dict(self, *args, **kwargs):
+        self._int8_weights.seen = None
+        return super().load_state_dict(*args, **kwargs)

@@ -171,7 +171,8 @@ int gnr_abi_version(void);
  * own declarations at load time (the ctypes binding does).  Unknown id -> 0. */
 enum { GNR_SIZEOF_PROBLEM = 0, GNR_SIZEOF_WEIGHTS = 1, GNR_SIZEOF_OUTPUTS = 2, GNR_SIZEOF_OUTPUT_GRADS = 3,
        GNR_SIZEOF_INPUT_GRADS = 4, GNR_SIZEOF_MERGE_PROBLEM = 5, GNR_SIZEOF_UPSAMPLE_PROBLEM = 6,
-       GNR_SIZEOF_UPSAMPLE_WEIGHTS = 7, GNR_SIZEOF_ROWS_PROBLEM = 8, GNR_SIZEOF_INT8_PROBLEM = 9 };
+       GNR_SIZEOF_UPSAMPLE_WEIGHTS = 7, GNR_SIZEOF_ROWS_PROBLEM = 8, GNR_SIZEOF_INT8_PROBLEM = 9,
+       GNR_SIZEOF_UPSAMPLE_INT8 = 10 };
 size_t gnr_sizeof(int which);
 
 /* Bytes of workspace `kind` needs for problem `p` with `n_streams` (1 or 2) weight sets. */
@@ -388,6 +389,28 @@ typedef struct GnrInt8Problem {
 
 size_t gnr_int8_linear_workspace_bytes(const GnrInt8Problem* p);     /* 0 + gnr_last_error() on bad input */
 int gnr_int8_linear(const GnrInt8Problem* p, void* workspace, size_t ws_bytes, void* stream);
+
+/* The upsampler's forward (gnr_upsample_fwd) with its 1x1 convolutions in 8 bits: inference, no saved state.  Weights as
+ * gnr_quantize_rows writes them (one scale an output channel); biases and the RGB branch from the fp32 GnrUpsampleWeights, whose
+ * up1_w / up2_w / feat_w are not read.  The map comes as p->x (fp32) or, with p->x NULL, as the cached rows x_q; the image is the
+ * same bit for bit for a map and for the rows gnr_quantize_rows makes of it. */
+typedef struct GnrUpsampleInt8 {
+    uint32_t struct_size, reserved;          /* = sizeof(GnrUpsampleInt8) of the caller */
+    const int8_t* up1_w[GNR_UPSAMPLE_MAX_BLOCKS];  int64_t up1_pitch[GNR_UPSAMPLE_MAX_BLOCKS];  const float* up1_s[GNR_UPSAMPLE_MAX_BLOCKS];
+    const int8_t* up2_w[GNR_UPSAMPLE_MAX_BLOCKS];  int64_t up2_pitch[GNR_UPSAMPLE_MAX_BLOCKS];  const float* up2_s[GNR_UPSAMPLE_MAX_BLOCKS];
+    const int8_t* feat_w[GNR_UPSAMPLE_MAX_BLOCKS]; int64_t feat_pitch[GNR_UPSAMPLE_MAX_BLOCKS]; const float* feat_s[GNR_UPSAMPLE_MAX_BLOCKS];
+    const int8_t* x_q;          /* NULL, or rows of a cache: strides and slots as in GnrInt8Problem             */
+    int64_t x_batch, x_pitch;
+    const float* x_scale;
+    int64_t x_scale_batch;
+    const int64_t* slots;
+    int64_t n_slots;
+} GnrUpsampleInt8;
+#define GNR_INIT_UPSAMPLE_INT8 { (uint32_t)sizeof(GnrUpsampleInt8) }
+
+size_t gnr_upsample_int8_workspace_bytes(const GnrUpsampleProblem* p, const GnrUpsampleInt8* q);
+int gnr_upsample_int8_fwd(const GnrUpsampleProblem* p, const GnrUpsampleWeights* w, const GnrUpsampleInt8* q, float* img, void* workspace,
+                          size_t ws_bytes, void* stream);
 
 const char* gnr_last_error(void);
 

@@ -1,0 +1,272 @@
+"""The upsampler in 8 bits (gazenerf_amd.upsample8) against a plain implementation that rounds where the definition says so.
+
+Up to the last block's output every value has ONE answer and is computed here on the CPU exactly as defined: 8-bit rows (sums of whole
+numbers, exact), an epilogue of named fp32 roundings, bf16 activations, a blur whose weights are powers of two in a fixed order.  What is
+left for a tolerance is the RGB branch: fp32 sums of C products in an order of their own (u = 2^-24: at most (C + 3) u of the sum of
+magnitudes), the upsampling of the running image (bilinear and blur: fewer than 16 roundings of a convex combination per level), and
+the sigmoid (slope at most 1/4, expf and the quotient within 4 u of a value below 1)."""
+import copy
+import ctypes as C
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+import gazenerf_amd as G
+from gazenerf_amd import _lib
+from gazenerf_amd.upsample import _channels, _expected_shapes, renderer_param_names
+from test_int8 import DEV, features, gen, ref_rows
+
+gpu = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def make_params(feat_nc, n_blocks, min_feat, seed, device=DEV):
+    g = gen(seed)
+    out = {}
+    for base, (o, k) in _expected_shapes(feat_nc, n_blocks, min_feat).items():
+        out[base + ".weight"] = (torch.randn(o, k, 1, 1, generator=g) * (2.0 / (o + k)) ** 0.5 * 1.5).to(device)
+        out[base + ".bias"] = (torch.randn(o, generator=g) * 0.1).to(device)
+    return {n: out[n] for n in renderer_param_names(n_blocks)}
+
+
+def product(q, s, w, b):
+    """fp32 roundings of the epilogue: fl(fl(sum) * s), one fused multiply-add, the leaky product; then bf16.  q, w whole numbers in float64."""
+    wq, ws = ref_rows(w.reshape(w.shape[0], -1))
+    t = (q @ wq.t()).float() * s.unsqueeze(-1)
+    v = (t.double() * ws.double() + b.cpu().double()).float()
+    return torch.maximum(v, v * torch.tensor(0.2)).bfloat16()
+
+
+def up_image(rgb):
+    """blur(bilinear x2) of [B, 3, S, S] in 64 bits."""
+    x = F.interpolate(rgb, scale_factor=2, mode="bilinear", align_corners=False)
+    x = F.pad(x, (1, 1, 1, 1), mode="reflect")
+    k = torch.tensor([1.0, 2.0, 1.0], dtype=x.dtype)
+    k = (k[:, None] * k[None, :] / 16).view(1, 1, 3, 3).expand(3, 1, 3, 3)
+    return F.conv2d(x, k, groups=3)
+
+
+def reference(rows, scale, params, S, n_blocks, min_feat, final):
+    """rows float64 [B, P, C], scale float32 [B, P] -> (image float64, bound)."""
+    B, P, Cn = rows.shape
+    ch = _channels(Cn, n_blocks, min_feat)
+    get = lambda n: params[n].detach().cpu()
+
+    def rgb_conv(v, level):
+        w, b = get("feat_2_rgb_list.%d.weight" % level).reshape(3, -1).double(), get("feat_2_rgb_list.%d.bias" % level).double()
+        y = v.double() @ w.t() + b
+        mag = v.double().abs() @ w.abs().t() + b.abs()
+        s = int(round(v.shape[1] ** 0.5))
+        shape = lambda t: t.transpose(1, 2).reshape(B, 3, s, s)
+        return shape(y), shape((v.shape[2] + 3) * U * mag)
+
+    q, s = rows, scale
+    res = None                                                              # None: the 8-bit rows are the residual
+    rgb, err = rgb_conv((rows.float() * scale.unsqueeze(-1)), 0)
+    rgb, err = up_image(rgb), up_image(err) + 16 * U * up_image(rgb.abs())
+    for i in range(n_blocks):
+        c = ch[i]
+        a1 = product(q, s, get("feat_upsample_list.%d.layer_1.weight" % i), get("feat_upsample_list.%d.layer_1.bias" % i))
+        a2 = product(*ref_rows(a1.float()), get("feat_upsample_list.%d.layer_2.weight" % i), get("feat_upsample_list.%d.layer_2.bias" % i))
+        idx = torch.arange(4 * c) % c
+        if res is None:
+            u = (q[..., idx] * s.double().unsqueeze(-1) + a2.double()).float()    # one fused multiply-add
+        else:
+            u = a2.float() + res.float()[..., idx]
+        u = u.reshape(B, S, S, c, 2, 2).permute(0, 3, 1, 4, 2, 5).reshape(B, c, 2 * S, 2 * S)
+        pad = F.pad(u, (1, 1, 1, 1), mode="reflect")
+        rowsum = (0.25 * pad[:, :, :-2] + 0.5 * pad[:, :, 1:-1]) + 0.25 * pad[:, :, 2:]
+        v = (0.25 * rowsum[..., :-2] + 0.5 * rowsum[..., 1:-1]) + 0.25 * rowsum[..., 2:]
+        S *= 2
+        v = v.permute(0, 2, 3, 1).reshape(B, S * S, c)
+        net = product(*ref_rows(v), get("feat_layers.%d.weight" % i), get("feat_layers.%d.bias" % i))
+        y, e = rgb_conv(net, i + 1)
+        rgb, err = rgb + y, err + e + U * (rgb.abs() + y.abs())
+        if i < n_blocks - 1:
+            rgb, err = up_image(rgb), up_image(err) + 16 * U * up_image(rgb.abs())
+            q, s = ref_rows(net.float())
+            res = net
+    if final:
+        rgb, err = torch.sigmoid(rgb), err / 4 + 4 * U
+    return rgb, err
+
+
+def check(img, rows, scale, params, S, n_blocks, min_feat, final):
+    ref, err = reference(rows, scale, params, S, n_blocks, min_feat, final)
+    assert img.shape == ref.shape
+    d = (img.cpu().double() - ref).abs()
+    bad = d > err
+    assert not bool(bad.any()), (int(bad.sum()), float((d / err).max()))
+
+
+# channels that a residual's four values wrap around in, one and several groups of threads a workgroup, rows of more channels than threads
+CASES = [(6, 2, 4, 16, 2, True), (33, 1, 8, 16, 1, False), (64, 2, 32, 16, 1, True), (129, 1, 32, 32, 2, True), (258, 2, 32, 16, 1, False),
+         (330, 1, 32, 16, 1, True), (1024, 1, 32, 16, 1, True), (48, 4, 8, 16, 1, True), (258, 3, 32, 64, 1, True)]
+
+
+@gpu
+@pytest.mark.parametrize("feat_nc, n_blocks, min_feat, S, B, final", CASES)
+def test_image_from_a_map(feat_nc, n_blocks, min_feat, S, B, final):
+    params = make_params(feat_nc, n_blocks, min_feat, feat_nc)
+    x = features((B, feat_nc, S, S), 1, feat_nc + S).to(DEV)
+    with torch.no_grad():
+        img = G.neural_render_int8(x, params, n_blocks, min_feat, final)
+    q, s = ref_rows(x.flatten(2).transpose(1, 2))
+    check(img, q, s, params, S, n_blocks, min_feat, final)
+
+
+@gpu
+def test_image_from_cached_rows():
+    """The same bits from the slots of a cache; padding slots are zero maps, slots outside the cache NaN images."""
+    params = make_params(33, 2, 8, 3)
+    x = features((3, 33, 16, 16), 1, 5).to(DEV)
+    cache = G.FeatureMapCache(5, 33, 256, device=DEV)
+    cache.write([4, 0, 2], x)
+    with torch.no_grad():
+        direct = G.neural_render_int8(x, params, 2, 8)
+        slots = torch.tensor([2, -1, 4, 5, 0, 2], device=DEV)
+        img = G.neural_render_int8(None, params, 2, 8, cache=cache, slots=slots)
+        zero = G.neural_render_int8(torch.zeros_like(x[:1]), params, 2, 8)
+        never = G.neural_render_int8(None, params, 2, 8, cache=cache, slots=torch.tensor([1], device=DEV))
+        view = G.FeatureMapCache(5, 33, 256, device=DEV)                         # rows the product cannot read in place
+        view.q, view.scale = cache.q.clone()[..., :33].contiguous(), cache.scale
+        odd = G.neural_render_int8(None, params, 2, 8, cache=view, slots=slots)
+    assert torch.equal(img[[0, 2, 4, 5]], direct[[2, 0, 1, 2]]) and torch.equal(img[1], zero[0])
+    assert bool(torch.isnan(img[3]).all()) and bool(torch.isnan(never).all())
+    assert torch.equal(odd.nan_to_num(), img.nan_to_num())
+
+
+def small_renderer(**kw):
+    torch.manual_seed(0)
+    return G.NeuralRendererAMD(feat_nc=36, featmap_size=16, img_size=64, min_feat=8, **kw).to(DEV)
+
+
+@gpu
+def test_module_replays_and_follows_its_parameters():
+    """graph_inference: every replay equals the eager call on the inputs and parameters it saw -- after an in-place update (an optimizer's), a
+    new storage, a load_state_dict -- with eager calls in between and two input shapes alive."""
+    net = small_renderer(precision="int8")
+    eager = lambda x: G.neural_render_int8(x, {k: v for k, v in net.named_parameters() if k != "bg_featmap"}, 2, 8)
+    xs = [features((b, 36, 16, 16), 1, b).to(DEV) for b in (1, 2, 1, 2, 1)]
+    with torch.no_grad():
+        for x in xs:
+            assert torch.equal(net(x), eager(x))
+        assert net._graphed8.captures == 2 and net._graphed8.replays == 5 and net._int8_weights.quantised == 1
+        before = net(xs[0])
+        net.feat_layers[0].weight.mul_(1.5)                                     # counted by torch
+        net.feat_2_rgb_list[1].bias.add_(0.25)                                  # read in place by the graph
+        for x in xs[:3]:
+            assert torch.equal(net(x), eager(x))
+        assert not torch.equal(net(xs[0]), before) and net._int8_weights.quantised == 2 and net._graphed8.captures == 2
+        state = {k: v * 0.5 for k, v in net.state_dict().items()}
+        net.load_state_dict(state)
+        assert torch.equal(net(xs[0]), eager(xs[0]))
+        net.feat_layers[1].weight.data.copy_(net.feat_layers[1].weight.data * 2)   # not counted: train() / eval() looks again
+        net.eval()
+        assert torch.equal(net(xs[1]), eager(xs[1]))
+        twin = copy.deepcopy(net)
+        assert torch.equal(twin(xs[0]), net(xs[0])) and twin._graphed8 is not net._graphed8
+    with torch.inference_mode():
+        assert torch.equal(net(xs[3]), eager(xs[3]))
+
+
+@gpu
+def test_module_renders_cached_views():
+    net = small_renderer()                                                       # fp32 by itself; cached views are 8-bit
+    x = features((3, 36, 16, 16), 1, 9).to(DEV)
+    cache = G.FeatureMapCache(4, 36, 256, device=DEV)
+    cache.write([0, 1, 3], x)
+    params = {k: v for k, v in net.named_parameters() if k != "bg_featmap"}
+    with torch.no_grad():
+        want = G.neural_render_int8(x, params, 2, 8)
+        for slots in ([3, 0], 1, torch.tensor([0, 3], device=DEV), [0, 1]):
+            img = net.render_cached(cache, slots)
+            idx = {0: 0, 1: 1, 3: 2}
+            assert torch.equal(img, want[[idx[int(s)] for s in cache.slots(slots)]])
+        cache.write(1, x[:1])                                                    # the graph reads the cache in place
+        assert torch.equal(net.render_cached(cache, [0, 1]), want[[0, 0]])
+        with pytest.raises(IndexError):
+            net.render_cached(cache, [4])
+        with pytest.raises(ValueError, match="cache holds"):
+            net.render_cached(G.FeatureMapCache(4, 35, 256, device=DEV), [0])
+    with pytest.raises(RuntimeError, match="no backward"):
+        net.render_cached(cache, [0])
+    with pytest.raises(RuntimeError, match="no backward"):
+        small_renderer(precision="int8")(x)
+
+
+@gpu
+def test_network_caches_and_renders_views():
+    """GazeNeRFNetAMD: cache_views renders and keeps the merged maps, render_views turns them into the images of its own forward in 8 bits."""
+    from gazenerf_amd import synth
+    torch.manual_seed(1)
+    net = G.GazeNeRFNetAMD(featmap_size=16, pred_img_size=32, num_sample_coarse=32, renderer_precision="int8").to(DEV)
+    p = {k: v.to(DEV) for k, v in synth.synth_problem(16, batch=2, camera="3", seed=2).items()}
+    args = dict(batch_xy=p["xy"], shape_code=p["shape_code"], appea_code=p["appea_code"], gaze_code=p["gaze"], batch_Rmats=p["R"], batch_Tvecs=p["T"],
+                batch_inv_inmats=p["Kinv"])
+    cache = G.FeatureMapCache(3, net.featmap_nc, 256, device=DEV)
+    net.cache_views(cache, [2, 0], **args)
+    img = net.render_views(cache, [0, 2, 0])
+    with torch.no_grad():
+        full = net("test", batch_uv=None, bg_code=None, **args)["coarse_dict"]
+    assert torch.equal(img, full["merge_img"][[1, 0, 1]])
+    assert bool(torch.isfinite(img).all())
+
+
+# ---- CPU: refusals ---------------------------------------------------------------------------------------------------------------
+def test_refusals(lib_built):
+    with pytest.raises(ValueError, match="precision"):
+        G.NeuralRendererAMD(precision="int4")
+    net = G.NeuralRendererAMD(feat_nc=24, featmap_size=16, img_size=32, min_feat=8, precision="int8")
+    with pytest.raises(RuntimeError, match="no backward"):
+        net(torch.zeros(1, 24, 16, 16))
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA/ROCm"):
+        net(torch.zeros(1, 24, 16, 16))
+    params = {k: v for k, v in net.named_parameters() if k != "bg_featmap"}
+    with torch.no_grad(), pytest.raises(ValueError, match="either a feature map or a cache"):
+        G.neural_render_int8(None, params, 1, 8)
+    cache = G.FeatureMapCache(2, 24, 256, device="cpu")
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA/ROCm"):
+        G.neural_render_int8(None, params, 1, 8, cache=cache, slots=torch.zeros(1, dtype=torch.int64))
+
+
+def test_c_entry_refuses(lib_built):
+    lib = _lib.load()
+
+    def args(prob={}, rows={}):
+        p, q, w = _lib.GnrUpsampleProblem(), _lib.GnrUpsampleInt8(), _lib.GnrUpsampleWeights()
+        p.batch, p.feat_nc, p.featmap_size, p.n_blocks, p.min_feat, p.final_sigmoid, p.x = 1, 24, 16, 1, 8, 1, 4096
+        for s in ("up1", "up2", "feat"):
+            getattr(q, s + "_w")[0], getattr(q, s + "_pitch")[0], getattr(q, s + "_s")[0] = 4096, 128, 4096
+            getattr(w, s + "_b")[0] = 4096
+        for i in range(2):
+            w.rgb_w[i], w.rgb_b[i] = 4096, 4096
+        for k, v in prob.items():
+            setattr(p, k, v)
+        for k, v in rows.items():
+            setattr(q, k, v)
+        return p, q, w
+
+    cached = dict(x_q=4096, x_batch=8192, x_pitch=32, x_scale=4096, x_scale_batch=256)
+    bad = [(dict(struct_size=3), {}, "struct_size"), ({}, dict(struct_size=3), "struct_size"), (dict(batch=0), {}, "batch"), (dict(featmap_size=24), {}, "power of two"),
+           (dict(feat_nc=1025), {}, "1024"), (dict(x=None), {}, "x is NULL"), (dict(feat_nc=3, min_feat=1), {}, "at least 4"), ({}, cached, "both x and x_q"), (dict(batch=65536), {}, "65536"),
+           (dict(x=None), dict(cached, x_scale=None), "x_scale"), (dict(x=None), dict(cached, x_pitch=24), "16-byte"), (dict(x=None), dict(cached, x_pitch=16), "16-byte"),
+           (dict(x=None), dict(cached, x_q=4104), "16-byte"), (dict(x=None), dict(cached, slots=4096), "n_slots")]
+    for prob, rows, word in bad:
+        p, q, w = args(prob, rows)
+        assert lib.gnr_upsample_int8_workspace_bytes(C.byref(p), C.byref(q)) == 0 and word in lib.gnr_last_error().decode(), (prob, rows, lib.gnr_last_error())
+        assert lib.gnr_upsample_int8_fwd(C.byref(p), C.byref(w), C.byref(q), 4096, 4096, 1 << 30, None) != 0
+    p, q, w = args()
+    need = lib.gnr_upsample_int8_workspace_bytes(C.byref(p), C.byref(q))
+    assert need > 0
+    for a, word in (((C.byref(w), C.byref(q), None, 4096, need), "image"), ((None, C.byref(q), 4096, 4096, need), "weights"),
+                    ((C.byref(w), C.byref(q), 4096, 4096, need - 1), "workspace"), ((C.byref(w), C.byref(q), 4096, 4104, need), "256-byte")):
+        assert lib.gnr_upsample_int8_fwd(C.byref(p), *a, None) != 0 and word in lib.gnr_last_error().decode()
+    for field in ("up1_w", "up2_s", "feat_w"):
+        p, q, w = args()
+        getattr(q, field)[0] = None
+        assert lib.gnr_upsample_int8_fwd(C.byref(p), C.byref(w), C.byref(q), 4096, 4096, need, None) != 0
+    p, q, w = args()
+    w.rgb_b[1] = None
+    assert lib.gnr_upsample_int8_fwd(C.byref(p), C.byref(w), C.byref(q), 4096, 4096, need, None) != 0
