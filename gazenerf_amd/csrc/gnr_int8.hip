@@ -21,7 +21,7 @@ struct Int8Args {
     void* y;
     long P, N;                    // rows per batch entry, all rows
     int K, O, leaky;
-    const void* xf; long xf_pitch; // floating rows that the few-rows kernel quantises itself
+    const void* xf; long xf_batch, xf_pitch;     // floating rows or maps that a kernel quantises itself
     int flat;                     // no slots, and every row of x a.x_pitch behind the one before (scales alike)
 };
 
@@ -386,6 +386,191 @@ __global__ __launch_bounds__(256) void int8_few_kernel(const Int8Args a) {
 }
 
 // ---------------------------------------------------------------------------------------------
+// floating x, few outputs or few rows: quantise and multiply in one launch.  A workgroup turns 32 NMT rows of x into 8-bit rows in LDS (maps: as
+// quant_maps_kernel reads them; rows: eight lanes a row) and multiplies them with `span` tiles of 32 outputs, the weights read from L2
+// fragment by fragment, so neither the 8-bit rows nor a second launch pass through memory.  A wave takes one 32-row tile (wave % NMT) and
+// every (4 / NMT)th output tile.  See the rule at int8_fuse.
+// ---------------------------------------------------------------------------------------------
+constexpr int FUSED_MAX_K = 512;
+__host__ __device__ constexpr int fused_ld(int K) { return (K + 31) / 32 * 32 + 16; }       // a row in LDS; + 16: eight lanes hit different columns
+
+template <typename X, typename T, bool CF, int NMT>
+__global__ __launch_bounds__(256) void int8_fused_kernel(const Int8Args a, unsigned tiles, unsigned parts, int span) {
+    constexpr int V = Vec<X>::N, TP = 32 * NMT, NW = 4, NT = 64 * NW, U = 8;        // U: steps of K whose weights are in flight
+    extern __shared__ __attribute__((aligned(16))) char lds[];                 // [TP][ld] rows, then 4 KiB a wave for the epilogue
+    __shared__ unsigned amax[NW][CF ? TP : 1];
+    __shared__ __attribute__((aligned(16))) float xs[TP];
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, K = a.K, ld = fused_ld(K), K32 = (K + 31) & ~31;
+    const unsigned blk = xcd_block(gridDim.x), at = blk / parts;               // a tile's parts of the outputs are neighbours
+    const long b = CF ? at / tiles : 0, P = CF ? a.P : a.N, p0 = (long)(CF ? at % tiles : at) * TP;
+    const int rows = P - p0 < TP ? (int)(P - p0) : TP;
+    constexpr int OW = NW / NMT;                               // waves that share a 32-row tile
+    const int mt = wave % NMT, steps = K32 / 32, half = lane >> 5, K16 = (K + 15) & ~15, o_tiles = (a.O + 31) / 32;
+    const int ot0 = (int)(blk % parts) * span + wave / NMT, ot1 = (int)(blk % parts) * span + span < o_tiles ? (int)(blk % parts) * span + span : o_tiles;
+    i32x4 w[U];
+    auto weights = [&](int ot, int s0) {
+        const int o = 32 * ot + (lane & 31) < a.O ? 32 * ot + (lane & 31) : a.O - 1;
+        const int8_t* wp = a.w + (long)o * a.w_pitch;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = 32 * (s0 + u) + 16 * half;
+            if (s0 + u < steps) w[u] = *(const i32x4*)(wp + (k < K16 ? k : K16 - 16));     // never behind the row
+        }
+    };
+    if (NMT == 1 && ot0 < ot1) weights(ot0, 0);                // under the quantisation (larger tiles: the registers cost more than it gives)
+
+    if constexpr (CF) {                                        // maps: element (b, c, p) at xf[b xf_batch + c xf_pitch + p]
+        constexpr int LPX = TP / V, G = NT / LPX, R = 4;
+        const int l = tid % LPX, g = tid / LPX;
+        const X* xb = (const X*)a.xf + b * a.xf_batch + p0 + l * V;
+        const int nv = rows - l * V;
+        Raw16 x[R][4];
+        unsigned m[4] = {};
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int c = 4 * (r * G + g) + e;
+                x[r][e] = c < K && nv > 0 ? load_raw(xb + (long)c * a.xf_pitch, nv) : Raw16{};
+            }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) m[w] = max_bits<X>(m[w], x[r][e].w[w]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+#pragma unroll
+            for (int i = LPX; i < 64; i <<= 1) m[w] = max_bits<X>(m[w], (unsigned)__shfl_xor((int)m[w], i));
+            if (lane < LPX) amax[wave][l * 4 + w] = m[w];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+            for (int i = 0; i < NW; ++i) m[w] = max_bits<X>(m[w], amax[i][l * 4 + w]);
+        float per[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float s;
+            row_scale(__float_as_uint(raw_value<X>(m, v)), s, per[v]);
+            if (g == 0) xs[l * V + v] = s;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int c = 4 * (r * G + g);
+            if (c < K32)
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    *(unsigned*)(lds + (l * V + v) * ld + c) = pack4(row_step(raw_value<X>(x[r][0].w, v), per[v]), row_step(raw_value<X>(x[r][1].w, v), per[v]),
+                                                                     row_step(raw_value<X>(x[r][2].w, v), per[v]), row_step(raw_value<X>(x[r][3].w, v), per[v]));
+        }
+    } else {                                                   // rows
+        constexpr int LPR = NT / 32, J = FUSED_MAX_K / (LPR * V) > 0 ? FUSED_MAX_K / (LPR * V) : 1;      // 32 rows at a time
+        const int l = tid % LPR;
+#pragma unroll 1
+        for (int t = 0; t < NMT; ++t) {
+            const int i = 32 * t + tid / LPR;
+            const X* row = (const X*)a.xf + (p0 + (i < rows ? i : rows - 1)) * a.xf_pitch;
+            Raw16 x[J];
+            unsigned m[4] = {};
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int c = (j * LPR + l) * V;
+                x[j] = c < K ? load_raw(row + c, K - c) : Raw16{};
+            }
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) m[w] = max_bits<X>(m[w], x[j].w[w]);
+            m[0] = max_bits<X>(max_bits<X>(m[0], m[1]), max_bits<X>(m[2], m[3]));
+#pragma unroll
+            for (int e = 1; e < LPR; e <<= 1) m[0] = max_bits<X>(m[0], (unsigned)__shfl_xor((int)m[0], e));
+            if constexpr (sizeof(X) == 2) m[0] = max_bits<X>(m[0], m[0] >> 16);
+            float s, per;
+            row_scale(__float_as_uint(raw_value<X>(m, 0)), s, per);
+            if (l == 0) xs[i] = s;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int c = (j * LPR + l) * V;
+                if (c < K32) {
+                    unsigned q[V / 4];
+#pragma unroll
+                    for (int w = 0; w < V / 4; ++w)
+                        q[w] = pack4(row_step(raw_value<X>(x[j].w, 4 * w), per), row_step(raw_value<X>(x[j].w, 4 * w + 1), per),
+                                     row_step(raw_value<X>(x[j].w, 4 * w + 2), per), row_step(raw_value<X>(x[j].w, 4 * w + 3), per));
+                    __builtin_memcpy(__builtin_assume_aligned(lds + i * ld + c, V), q, V);
+                }
+            }
+        }
+    }
+    __syncthreads();
+
+    const char* xr = lds + (32 * mt + (lane & 31)) * ld + 16 * half;
+    float* turn = (float*)(lds + TP * ld) + wave * 1024;
+    const long M = CF ? a.P : a.O;
+    T* yb = (T*)a.y + (CF ? b * (long)a.O * a.P : 0);
+    for (int ot = ot0; ot < ot1; ot += OW) {
+        const int o = 32 * ot + (lane & 31) < a.O ? 32 * ot + (lane & 31) : a.O - 1;
+        const float wsc = a.ws[o], wb = a.bias ? a.bias[o] : 0.0f;
+        i32x16 acc = {};
+        for (int s0 = 0; s0 < steps; s0 += U) {
+            if (NMT > 1 || s0 || ot != ot0) weights(ot, s0);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = 32 * (s0 + u);
+                if (s0 + u >= steps) continue;
+                const i32x4 xv = *(const i32x4*)(xr + k);      // the bytes behind K are 0 here: what stands there in w does not count
+                acc = CF ? __builtin_amdgcn_mfma_i32_32x32x32_i8(xv, w[u], acc, 0, 0, 0) : __builtin_amdgcn_mfma_i32_32x32x32_i8(w[u], xv, acc, 0, 0, 0);
+            }
+        }
+        // m: pixels (CF) or outputs; n = lane % 32: outputs (CF) or rows.  The 32 x 32 values turn in LDS so that stores run along m.
+        const int nr = lane & 31;
+        const float xn = CF ? 0.0f : xs[32 * mt + nr];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            fv4 v;
+            const int ml = 8 * q + 4 * half;
+            fv4 sm, bm;
+            if constexpr (CF) {
+                sm = *(const fv4*)(xs + 32 * mt + ml);
+                bm = fv4{wb, wb, wb, wb};
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    sm[r] = __shfl(wsc, ml + r);
+                    bm[r] = __shfl(wb, ml + r);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                v[r] = fmaf((float)acc[4 * q + r] * (CF ? sm[r] : xn), CF ? wsc : sm[r], bm[r]);
+                if (a.leaky) v[r] = leak(v[r]);
+            }
+            *(fv4*)(turn + nr * 32 + 4 * ((ml >> 2) ^ (nr & 7))) = v;
+        }
+        constexpr int TV = Vec<T>::N, PPR = 32 / TV;           // 16-byte pieces of T in a row of 32
+#pragma unroll
+        for (int it = 0; it < 32 * PPR / 64; ++it) {
+            const int row = it * (64 / PPR) + lane / PPR, m = (lane % PPR) * TV;
+            Vec<T> out;
+#pragma unroll
+            for (int i = 0; i < TV; i += 4) {
+                const fv4 v = *(const fv4*)(turn + row * 32 + 4 * (((m + i) >> 2) ^ (row & 7)));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) out.v[i + r] = (T)v[r];
+            }
+            const long n = CF ? 32 * ot + row : p0 + 32 * mt + row, mg = CF ? p0 + 32 * mt + m : 32 * ot + m;
+            const long left = M - mg;
+            if (n < (CF ? (long)a.O : a.N) && left > 0) {
+                if (CF && sizeof(T) == 4) store_part<true>(yb + n * M + mg, out, left < TV ? (int)left : TV);
+                else store_part(yb + n * M + mg, out, left < TV ? (int)left : TV);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
 static int check_int8(const GnrInt8Problem* p) {
@@ -417,9 +602,32 @@ static int check_int8(const GnrInt8Problem* p) {
     return 0;
 }
 
-// floating rows that the few-rows kernel takes as they are
-static bool int8_fused(const GnrInt8Problem* p) {
-    return p->x_type != GNR_I8 && !p->x_channels_first && !p->y_channels_first && p->batch == 1 && p->n_pix <= FEW_FUSED && p->k <= FEW_FUSED_K;
+// Which kernel takes floating x as it is (FUSE_NONE: x is quantised into the workspace first), us by fused / two launches:
+//   FUSE_FEW  rows that the few-rows kernel takes
+//   1 2 4     int8_fused_kernel with that many 32-row tiles a workgroup
+// Up to 128 outputs a workgroup multiplies with all of them: 1 + 1 / 128 .. reads of x, no 8-bit rows in memory (262144 x 64 -> 32, fp32
+// maps: 18.8 / 27.9), with as many row tiles as keep four waves busy, fewer where a row of K does not fit a thread's registers.
+// Beyond, every workgroup takes four output tiles and the rows are quantised again for each: only while there is a CU for every workgroup,
+// when what counts is one launch instead of two (88 x 456 -> 1701, fp16: 6.7 / 10.4; 4096 x 258 -> 516, 640 workgroups: 11.5 / 10.1).
+enum { FUSE_NONE = 0, FUSE_FEW = 8 };
+static int fused_parts(long O, int nmt, int* span) {
+    const long o_tiles = (O + 31) / 32;
+    *span = (int)(O <= 128 ? o_tiles : 4 / nmt);
+    return (int)((o_tiles + *span - 1) / *span);
+}
+static int int8_fuse(const GnrInt8Problem* p) {
+    if (p->x_type == GNR_I8 || p->x_channels_first != p->y_channels_first) return FUSE_NONE;
+    const bool cf = p->x_channels_first != 0;
+    const long N = (long)p->batch * p->n_pix;
+    if (!cf && p->batch == 1 && N <= FEW_FUSED && p->k <= FEW_FUSED_K) return FUSE_FEW;
+    if ((!cf && p->batch != 1) || p->k > FUSED_MAX_K) return FUSE_NONE;
+    const int vec = p->x_type == GNR_F32 ? 4 : 8;
+    int nmt = p->o <= 32 ? 4 : (p->o <= 64 ? 2 : 1), span;
+    while (cf && nmt > 1 && p->k > 32 * vec * 4 / nmt) nmt /= 2;               // maps: 4 quads of channels a thread
+    if (cf && p->k > 32 * vec * 4 / nmt) return FUSE_NONE;
+    const long groups = cf ? p->batch * ((p->n_pix + 32 * nmt - 1) / (32 * nmt)) : (N + 32 * nmt - 1) / (32 * nmt), parts = fused_parts(p->o, nmt, &span);
+    if (groups * parts >= (1L << 31)) return FUSE_NONE;
+    return p->o <= 128 || groups * parts <= 256 ? nmt : FUSE_NONE;
 }
 
 struct Int8Ws {
@@ -427,7 +635,7 @@ struct Int8Ws {
 };
 static Int8Ws int8_ws(const GnrInt8Problem* p) {                     // floating x: its rows and their scales
     Int8Ws w{};
-    if (p->x_type == GNR_I8 || int8_fused(p)) return w;
+    if (p->x_type == GNR_I8 || int8_fuse(p)) return w;
     const size_t n = (size_t)p->batch * (size_t)p->n_pix;
     w.q_pitch = ((size_t)p->k + 63) & ~(size_t)63;                   // a stage of a row never crosses a line: 28672 x 516 -> 1032 41 -> 38 us
     w.q_bytes = (n * w.q_pitch + 255) & ~(size_t)255;
@@ -475,11 +683,24 @@ template <typename T, bool CF> static int launch_int8(const Int8Args& a, long ba
     if (t128 >= 256) return launch_tile<T, CF, 2, 2, 2, 2, 3>(a, batch, st);
     return launch_tile<T, CF, 2, 2, 1, 1, 4>(a, batch, st);
 }
-template <typename X> static void launch_fused(const Int8Args& a, int y_type, hipStream_t st) {
-    if (y_type == GNR_F32) launch_few<X, float, false, 1>(a, st);
-    else if (y_type == GNR_BF16) launch_few<X, __bf16, false, 1>(a, st);
-    else launch_few<X, _Float16, false, 1>(a, st);
+template <typename X, typename T, bool CF, int NMT> static void launch_fused_tile(const Int8Args& a, long batch, hipStream_t st) {
+    int span;
+    const long P = CF ? a.P : a.N, tiles = (P + 32 * NMT - 1) / (32 * NMT), parts = fused_parts(a.O, NMT, &span), blocks = (CF ? tiles * batch : tiles) * parts;
+    hipLaunchKernelGGL((int8_fused_kernel<X, T, CF, NMT>), dim3((unsigned)blocks), dim3(256), 32 * NMT * fused_ld(a.K) + 4 * 4096, st, a, (unsigned)tiles,
+                       (unsigned)parts, span);
 }
+template <typename X, typename T> static void launch_fused_type(const Int8Args& a, long batch, bool cf, int how, hipStream_t st) {
+    if (how == FUSE_FEW) launch_few<X, T, false, 1>(a, st);
+    else if (how == 1) cf ? launch_fused_tile<X, T, true, 1>(a, batch, st) : launch_fused_tile<X, T, false, 1>(a, batch, st);
+    else if (how == 2) cf ? launch_fused_tile<X, T, true, 2>(a, batch, st) : launch_fused_tile<X, T, false, 2>(a, batch, st);
+    else cf ? launch_fused_tile<X, T, true, 4>(a, batch, st) : launch_fused_tile<X, T, false, 4>(a, batch, st);
+}
+template <typename X> static void launch_fused(const Int8Args& a, int y_type, long batch, bool cf, int how, hipStream_t st) {
+    if (y_type == GNR_F32) launch_fused_type<X, float>(a, batch, cf, how, st);
+    else if (y_type == GNR_BF16) launch_fused_type<X, __bf16>(a, batch, cf, how, st);
+    else launch_fused_type<X, _Float16>(a, batch, cf, how, st);
+}
+
 }  // namespace gnr
 
 using namespace gnr;
@@ -502,11 +723,12 @@ int gnr_int8_linear(const GnrInt8Problem* p, void* workspace, size_t ws_bytes, v
     if (p->x_type == GNR_I8) {
         a.x = (const int8_t*)p->x; a.x_batch = p->x_batch; a.x_pitch = p->x_stride; a.xs = p->x_scale; a.xs_batch = p->x_scale_batch;
         a.slots = p->slots; a.n_slots = p->n_slots;
-    } else if (int8_fused(p)) {
-        a.xf = p->x; a.xf_pitch = p->x_stride;
-        if (p->x_type == GNR_F32) launch_fused<float>(a, p->y_type, st);
-        else if (p->x_type == GNR_BF16) launch_fused<__bf16>(a, p->y_type, st);
-        else launch_fused<_Float16>(a, p->y_type, st);
+    } else if (const int how = int8_fuse(p)) {
+        const bool cf = p->y_channels_first != 0;
+        a.xf = p->x; a.xf_batch = p->x_batch; a.xf_pitch = p->x_stride;
+        if (p->x_type == GNR_F32) launch_fused<float>(a, p->y_type, p->batch, cf, how, st);
+        else if (p->x_type == GNR_BF16) launch_fused<__bf16>(a, p->y_type, p->batch, cf, how, st);
+        else launch_fused<_Float16>(a, p->y_type, p->batch, cf, how, st);
         const hipError_t e = hipGetLastError();
         return e == hipSuccess ? 0 : fail("gnr_int8_linear: launch failed: %s", hipGetErrorString(e));
     } else {

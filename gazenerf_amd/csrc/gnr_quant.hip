@@ -26,16 +26,6 @@ __global__ __launch_bounds__(1024) void quant_maps_kernel(const GnrRowsProblem p
     const int NT = (int)blockDim.x, G = NT / LPX, tid = (int)threadIdx.x, l = tid % LPX, g = tid / LPX;
     const unsigned at = xcd_block(gridDim.x);
     const long b = at / tiles, p0 = tile_start(at % tiles, TP, p.n_pix);
-    long slot = b;
-    if (p.slots) {
-        const SlotRef ref = slot_of(p.slots, p.n_slots, b);
-        if (ref.state) return;                              // the whole workgroup
-        slot = ref.slot;
-        // the same slot again later in the list: the LAST map stays, whichever workgroup runs first
-        int again = 0;
-        for (long j = b + 1 + tid; j < p.batch; j += NT) again |= p.slots[j] == slot;
-        if (__syncthreads_or(again)) return;
-    }
     unsigned* tile = smem;                                  // [TP][ld]: one quad of channels of one pixel a word
     unsigned* amax = smem + TP * ld;                        // [NT / 64][LPX][4]
     const int C = p.channels;
@@ -58,9 +48,20 @@ __global__ __launch_bounds__(1024) void quant_maps_kernel(const GnrRowsProblem p
                 else x[r][e] = Raw16{};
             }
     };
+    load(0);
+    long slot = b;
+    if (p.slots) {
+        const SlotRef ref = slot_of(p.slots, p.n_slots, b);
+        if (ref.state) return;                              // the whole workgroup; x is on its way meanwhile
+        slot = ref.slot;
+        // the same slot again later in the list: the LAST map stays, whichever workgroup runs first
+        int again = 0;
+        for (long j = b + 1 + tid; j < p.batch; j += NT) again |= p.slots[j] == slot;
+        if (__syncthreads_or(again)) return;
+    }
     unsigned a[4] = {};
     for (int k = 0; k < n_chunk; ++k) {
-        load(k * step);
+        if (k) load(k * step);
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -189,10 +190,12 @@ template <typename T> __device__ __forceinline__ T row_value(int q, float s) {
 // ---------------------------------------------------------------------------------------------
 template <typename T, int LPX>
 __global__ __launch_bounds__(256) void read_maps_kernel(const GnrRowsProblem p, unsigned tiles, int ld, int step) {
-    constexpr int V = Vec<T>::N, TP = LPX * V, G = 256 / LPX, U = 4;
+    constexpr int V = Vec<T>::N, TP = LPX * V, U = 4;
     extern __shared__ unsigned smem[];                      // [TP][ld]
-    const int tid = (int)threadIdx.x, l = tid % LPX, g = tid / LPX;
-    const unsigned at = blockIdx.x;
+    const int NT = (int)blockDim.x, G = NT / LPX, tid = (int)threadIdx.x, l = tid % LPX, g = tid / LPX;
+    // maps whose channels are whole lines: past the caches, any order.  Others: neighbouring tiles share lines, which one L2 puts together
+    const bool lines = (p.x_stride * (long)sizeof(T)) % 128 == 0;
+    const unsigned at = lines ? blockIdx.x : xcd_block(gridDim.x);
     const long b = at / tiles, p0 = tile_start(at % tiles, TP, p.n_pix);
     const SlotRef ref = slot_of(p.slots, p.n_slots, b);
     const int C = p.channels, rows = p.n_pix - p0 < TP ? (int)(p.n_pix - p0) : TP;
@@ -208,16 +211,16 @@ __global__ __launch_bounds__(256) void read_maps_kernel(const GnrRowsProblem p, 
     for (int c0 = 0; c0 < C; c0 += step) {                  // once, unless the rows of a tile exceed the LDS
         const int cols = C - c0 < step ? C - c0 : step, per_row = (cols + 15) >> 4, n = ref.state ? 0 : rows * per_row;
         if (c0) __syncthreads();
-        for (int i0 = tid; i0 < n; i0 += 256 * U) {
+        for (int i0 = tid; i0 < n; i0 += NT * U) {
             Vec<int8_t> o[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int i = i0 + 256 * u, row = i / per_row, c = 16 * (i - row * per_row);
+                const int i = i0 + NT * u, row = i / per_row, c = 16 * (i - row * per_row);
                 if (i < n) o[u] = load_part(qb + row * p.q_pitch + c0 + c, cols - c);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int i = i0 + 256 * u, row = i / per_row, c = 16 * (i - row * per_row);
+                const int i = i0 + NT * u, row = i / per_row, c = 16 * (i - row * per_row);
                 if (i < n) __builtin_memcpy(__builtin_assume_aligned(smem + row * ld + (c >> 2), 16), &o[u], 16);
             }
         }
@@ -234,7 +237,11 @@ __global__ __launch_bounds__(256) void read_maps_kernel(const GnrRowsProblem p, 
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (4 * q + e < cols) store_part<true>(yb + (long)(c0 + 4 * q + e) * p.x_stride, y[e], nv);
+                if (4 * q + e < cols) {
+                    T* yp = yb + (long)(c0 + 4 * q + e) * p.x_stride;
+                    if (lines) store_part<true>(yp, y[e], nv);
+                    else store_part(yp, y[e], nv);
+                }
         }
     }
 }
@@ -288,12 +295,18 @@ template <typename T> static void quant_rows(const GnrRowsProblem& p, hipStream_
     const long total = (long)p.batch * p.n_pix;
     const int C = p.channels;
 #define GNR_ROWS(L, J) hipLaunchKernelGGL((quant_rows_kernel<T, L, J>), dim3((unsigned)((total + 256 / L - 1) / (256 / L))), dim3(256), 0, st, p, total)
-    if (C <= 16 * V) GNR_ROWS(16, 1);
-    else if (C <= 32 * V) GNR_ROWS(16, 2);
-    else if (C <= 64 * V) GNR_ROWS(16, 4);
-    else if (C <= 128 * V) GNR_ROWS(64, 2);
-    else if (C <= 256 * V) GNR_ROWS(64, 4);
-    else GNR_ROWS(64, 8);
+    switch ((C + 16 * V - 1) / (16 * V)) {                     // 16 lanes a row while eight pieces a lane hold it
+        case 1: GNR_ROWS(16, 1); break;
+        case 2: GNR_ROWS(16, 2); break;
+        case 3: GNR_ROWS(16, 3); break;
+        case 4: GNR_ROWS(16, 4); break;
+        case 5: GNR_ROWS(16, 5); break;
+        case 6: GNR_ROWS(16, 6); break;
+        case 7: case 8: GNR_ROWS(16, 8); break;
+        default:
+            if (C <= 256 * V) GNR_ROWS(64, 4);
+            else GNR_ROWS(64, 8);
+    }
 #undef GNR_ROWS
 }
 
@@ -315,7 +328,9 @@ template <typename T, int LPX> static void read_maps_lpx(const GnrRowsProblem& p
     constexpr int TP = LPX * Vec<T>::N;
     const unsigned tiles = (unsigned)((p.n_pix + TP - 1) / TP);
     const int step = p.channels < 1920 ? p.channels : 1920, ld = (step + 63) / 64 * 16 + 4;
-    hipLaunchKernelGGL((read_maps_kernel<T, LPX>), dim3(tiles * (unsigned)p.batch), dim3(256), sizeof(unsigned) * TP * ld, st, p, tiles, ld, step);
+    int nt = 64;                                               // a quad of channels a thread and turn: no more threads than quads
+    while (nt < 256 && (p.channels + 3) / 4 > nt / LPX) nt *= 2;
+    hipLaunchKernelGGL((read_maps_kernel<T, LPX>), dim3(tiles * (unsigned)p.batch), dim3((unsigned)nt), sizeof(unsigned) * TP * ld, st, p, tiles, ld, step);
 }
 template <typename T> static void read_maps(const GnrRowsProblem& p, hipStream_t st) { read_maps_lpx<T, sizeof(T) == 4 ? 8 : 4>(p, st); }
 
