@@ -258,6 +258,54 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void int8_tile_kernel(const Int8Ar
 // ---------------------------------------------------------------------------------------------
 constexpr int FEW_MAX = 64, FEW_FUSED = 16, FEW_FUSED_K = 4096;
 
+// floating rows -> 8-bit rows [n][ld] and scales in LDS, L lanes a row, eight pieces of 16 bytes a lane (longer rows are read twice)
+template <typename X, int L> __device__ __forceinline__ void few_rows(const X* xb, long pitch, int N, int K, int K64, int ld, char* lds, float* xsc) {
+    constexpr int V = Vec<X>::N, J = 8;
+    const int lane = (int)threadIdx.x % L;
+    for (int n = (int)threadIdx.x / L; n < N; n += 256 / L) {
+        const X* row = xb + (long)n * pitch;
+        Raw16 r[J];
+        unsigned m[4] = {};
+        auto get = [&](int j0) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int c = ((j0 + j) * L + lane) * V;
+                r[j] = c < K ? load_raw(row + c, K - c) : Raw16{};
+            }
+        };
+        const int pieces = (K + L * V - 1) / (L * V);
+        for (int j0 = 0; j0 < pieces; j0 += J) {
+            get(j0);
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) m[i] = max_bits<X>(m[i], r[j].w[i]);
+        }
+        m[0] = max_bits<X>(max_bits<X>(m[0], m[1]), max_bits<X>(m[2], m[3]));
+#pragma unroll
+        for (int i = 1; i < L; i <<= 1) m[0] = max_bits<X>(m[0], (unsigned)__shfl_xor((int)m[0], i));
+        if constexpr (sizeof(X) == 2) m[0] = max_bits<X>(m[0], m[0] >> 16);
+        float s, per;
+        row_scale(__float_as_uint(raw_value<X>(m, 0)), s, per);
+        if (lane == 0) xsc[n] = s;
+        for (int j0 = 0; j0 < pieces; j0 += J) {
+            if (pieces > J) get(j0);
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int c = ((j0 + j) * L + lane) * V;       // bytes behind K become 0: load_raw filled up with 0
+                if (c < K64) {
+                    unsigned q[V / 4];
+#pragma unroll
+                    for (int i = 0; i < V / 4; ++i)
+                        q[i] = pack4(row_step(raw_value<X>(r[j].w, 4 * i), per), row_step(raw_value<X>(r[j].w, 4 * i + 1), per),
+                                     row_step(raw_value<X>(r[j].w, 4 * i + 2), per), row_step(raw_value<X>(r[j].w, 4 * i + 3), per));
+                    __builtin_memcpy(__builtin_assume_aligned(lds + n * ld + c, V), q, V);
+                }
+            }
+        }
+    }
+}
+
 template <typename X, typename T, bool CF, int TT>
 __global__ __launch_bounds__(256) void int8_few_kernel(const Int8Args a) {
     constexpr bool FLOAT = !__is_same(X, int8_t);
@@ -294,50 +342,9 @@ __global__ __launch_bounds__(256) void int8_few_kernel(const Int8Args a) {
     };
     load(wave);                                                // under the quantisation
     if constexpr (FLOAT) {
-        constexpr int V = Vec<X>::N, J = FEW_FUSED_K / 2 / (64 * 4);           // 8 pieces a lane: 2048 values in fp32, 4096 in 16 bits
-        const X* xb = (const X*)a.xf;
-        for (int n = wave; n < N; n += 4) {
-            const X* row = xb + (long)n * a.xf_pitch;
-            Raw16 r[J];
-            unsigned m[4] = {};
-            auto get = [&](int j0) {
-#pragma unroll
-                for (int j = 0; j < J; ++j) {
-                    const int c = ((j0 + j) * 64 + lane) * V;
-                    r[j] = c < K ? load_raw(row + c, K - c) : Raw16{};
-                }
-            };
-            const int pieces = (K + 64 * V - 1) / (64 * V);
-            for (int j0 = 0; j0 < pieces; j0 += J) {
-                get(j0);
-#pragma unroll
-                for (int j = 0; j < J; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) m[i] = max_bits<X>(m[i], r[j].w[i]);
-            }
-            m[0] = max_bits<X>(max_bits<X>(m[0], m[1]), max_bits<X>(m[2], m[3]));
-#pragma unroll
-            for (int i = 1; i < 64; i <<= 1) m[0] = max_bits<X>(m[0], (unsigned)__shfl_xor((int)m[0], i));
-            if constexpr (sizeof(X) == 2) m[0] = max_bits<X>(m[0], m[0] >> 16);
-            float s, per;
-            row_scale(__float_as_uint(raw_value<X>(m, 0)), s, per);
-            if (lane == 0) xsc[n] = s;
-            for (int j0 = 0; j0 < pieces; j0 += J) {
-                if (pieces > J) get(j0);
-#pragma unroll
-                for (int j = 0; j < J; ++j) {
-                    const int c = ((j0 + j) * 64 + lane) * V;                  // bytes behind K become 0: load_raw filled up with 0
-                    if (c < nst * 64) {
-                        unsigned q[V / 4];
-#pragma unroll
-                        for (int i = 0; i < V / 4; ++i)
-                            q[i] = pack4(row_step(raw_value<X>(r[j].w, 4 * i), per), row_step(raw_value<X>(r[j].w, 4 * i + 1), per),
-                                         row_step(raw_value<X>(r[j].w, 4 * i + 2), per), row_step(raw_value<X>(r[j].w, 4 * i + 3), per));
-                        __builtin_memcpy(__builtin_assume_aligned(lds + n * ld + c, V), q, V);
-                    }
-                }
-            }
-        }
+        // one row a wave and turn, or four rows a wave where a sixteenth of one fits the same registers
+        if (N > 4 && K <= 16 * 8 * Vec<X>::N) few_rows<X, 16>((const X*)a.xf, a.xf_pitch, N, K, nst * 64, ld, lds, xsc);
+        else few_rows<X, 64>((const X*)a.xf, a.xf_pitch, N, K, nst * 64, ld, lds, xsc);
     }
     i32x4 acc[TT];
 #pragma unroll

@@ -311,19 +311,38 @@ Tensor rows3(const Tensor& t) {
     return m.stride(2) == 1 || k <= 1 ? m : m.contiguous();
 }
 int64_t stride_or(const Tensor& t, int64_t d, int64_t other) { return t.size(d) > 1 ? t.stride(d) : other; }
-// 8-bit rows [b, n, K] as a product reads them: on 16-byte boundaries, readable to the next multiple of 16
-Tensor pitched(const Tensor& q) {
-    const int64_t b = q.size(0), n = q.size(1), k = q.size(2), k16 = (k + 15) / 16 * 16;
-    bool ok = (k == 1 || q.stride(2) == 1) && (n <= 1 || (q.stride(1) % 16 == 0 && q.stride(1) >= k16)) &&
-              (b <= 1 || q.stride(0) % 16 == 0) && (uintptr_t)q.data_ptr() % 16 == 0;
-    if (ok && q.numel() != 0) {
-        const int64_t last = q.storage_offset() + (b - 1) * q.stride(0) + (n - 1) * q.stride(1) + k16;
-        ok = last <= (int64_t)q.storage().nbytes();
+// Rows [..., K] as (entries, rows of an entry) with two strides; `keep` holds the tensor the pointer belongs to.  2-D and 3-D tensors are
+// described as they are (a view costs half a microsecond), others through a reshape.
+struct RowsIn {
+    Tensor keep;
+    int64_t b = 1, n = 1, k = 0, sb = 0, sn = 0;
+};
+RowsIn rows_in(const Tensor& t) {
+    RowsIn r;
+    r.keep = t.dim() == 2 || t.dim() == 3 ? t : rows3(t);
+    const int64_t d = r.keep.dim();
+    r.k = r.keep.size(d - 1);
+    if (r.k > 1 && r.keep.stride(d - 1) != 1) r.keep = r.keep.contiguous();
+    r.n = r.keep.size(d - 2);
+    r.sn = r.keep.stride(d - 2);
+    if (d == 3) { r.b = r.keep.size(0); r.sb = r.keep.stride(0); }
+    return r;
+}
+// 8-bit rows as a product reads them: on 16-byte boundaries, readable to the next multiple of 16
+RowsIn rows8_in(const Tensor& t) {
+    RowsIn r = rows_in(t);
+    const int64_t k16 = (r.k + 15) / 16 * 16;
+    if (r.n <= 1) r.sn = k16;
+    if (r.b <= 1) r.sb = 0;
+    bool ok = r.sn % 16 == 0 && r.sn >= k16 && r.sb % 16 == 0 && (uintptr_t)r.keep.data_ptr() % 16 == 0;
+    if (ok && r.b > 0 && r.n > 0)
+        ok = r.keep.storage_offset() + (r.b - 1) * r.sb + (r.n - 1) * r.sn + k16 <= (int64_t)r.keep.storage().nbytes();
+    if (!ok) {
+        Tensor out = empty_rows(r.b, r.n, r.k, t.device());
+        out.copy_(r.keep.dim() == 3 ? r.keep : r.keep.unsqueeze(0));
+        r.keep = out; r.sn = row_pitch(r.k); r.sb = r.sn * r.n;
     }
-    if (ok) return q;
-    Tensor out = empty_rows(b, n, k, q.device());
-    out.copy_(q);
-    return out;
+    return r;
 }
 void* stream_of(const c10::Device& dev) { return (void*)c10::hip::getCurrentHIPStream(dev.index()).stream(); }
 
@@ -415,8 +434,10 @@ Tensor int8_linear(const Tensor& x, const Tensor& w_q, const Tensor& w_scale, co
     p.x_type = rows8 ? GNR_I8 : type_id(x.scalar_type(), "x");
     const at::ScalarType yt = type_of(out_type);
     p.y_type = (int32_t)out_type; p.leaky = leaky; p.y_channels_first = cf; p.k = (int32_t)k; p.o = (int32_t)o;
-    const Tensor w = pitched(w_q.unsqueeze(0)), ws_c = w_scale.contiguous();
-    Tensor b_c, xr, xs, sl;
+    const RowsIn w = rows8_in(w_q);
+    const Tensor ws_c = w_scale.contiguous();
+    Tensor b_c, xs, sl;
+    RowsIn xr;
     if (bias) {
         check_on(*bias, "bias", at::kFloat, 1, dev);
         TORCH_CHECK(bias->size(0) == o, "bias must have shape [", o, "], got ", bias->sizes());
@@ -431,12 +452,12 @@ Tensor int8_linear(const Tensor& x, const Tensor& w_q, const Tensor& w_scale, co
         check_on(*x_scale, "x_scale", at::kFloat, x.dim() - 1, dev);
         TORCH_CHECK(x_scale->sizes() == x.sizes().slice(0, x.dim() - 1), "x_scale must have the shape of x without its channels, got ",
                     x_scale->sizes());
-        xr = pitched(rows3(x));
-        b = xr.size(0); n = xr.size(1);
-        xs = x.dim() == 3 ? *x_scale : x_scale->reshape({b, n});
-        if (xs.size(1) > 1 && xs.stride(1) != 1) xs = xs.contiguous();
-        p.x_scale = xs.data_ptr<float>(); p.x_scale_batch = xs.stride(0);
-        p.x_batch = stride_or(xr, 0, 0); p.x_stride = stride_or(xr, 1, row_pitch(k));
+        xr = rows8_in(x);
+        b = xr.b; n = xr.n;
+        xs = x.dim() == 3 || x.dim() == 2 ? *x_scale : x_scale->reshape({b, n});
+        if (n > 1 && xs.stride(xs.dim() - 1) != 1) xs = xs.contiguous();
+        p.x_scale = xs.data_ptr<float>(); p.x_scale_batch = xs.dim() == 2 ? xs.stride(0) : 0;
+        p.x_batch = xr.sb; p.x_stride = xr.sn;
         if (slots) {
             check_on(*slots, "slots", at::kLong, 1, dev);
             TORCH_CHECK(b >= 1, "slots are given but x is empty: ", x.sizes());
@@ -448,10 +469,16 @@ Tensor int8_linear(const Tensor& x, const Tensor& w_q, const Tensor& w_scale, co
         else if (slots) shape = {b, n, o};
     } else {
         TORCH_CHECK(!x_scale && !slots, "x_scale and slots go with 8-bit x; floating x is quantised by the call");
-        xr = cf ? maps3(x) : rows3(x);
-        b = xr.size(0); n = xr.size(cf ? 2 : 1);
-        TORCH_CHECK(xr.size(cf ? 1 : 2) == k, "x has another number of channels than w_q: ", x.sizes(), ", ", w_q.sizes());
-        p.x_channels_first = cf; p.x_batch = xr.stride(0); p.x_stride = xr.stride(1);
+        if (cf) {
+            xr.keep = maps3(x);
+            xr.b = xr.keep.size(0); xr.k = xr.keep.size(1); xr.n = xr.keep.size(2); xr.sb = xr.keep.stride(0); xr.sn = xr.keep.stride(1);
+        } else {
+            TORCH_CHECK(x.dim() >= 1, "rows must be [..., K]");
+            xr = rows_in(x);
+        }
+        b = xr.b; n = xr.n;
+        TORCH_CHECK(xr.k == k, "x has another number of channels than w_q: ", x.sizes(), ", ", w_q.sizes());
+        p.x_channels_first = cf; p.x_batch = xr.sb; p.x_stride = xr.sn;
         if (cf) {
             shape = x.sizes().vec();
             shape[1] = o;
@@ -464,15 +491,15 @@ Tensor int8_linear(const Tensor& x, const Tensor& w_q, const Tensor& w_scale, co
     Tensor y = at::empty(shape, at::TensorOptions().dtype(yt).device(dev));
     if (y.numel() == 0) return y;
     TORCH_CHECK(b <= INT32_MAX, "too many entries: ", b);
-    p.batch = (int32_t)b; p.n_pix = n; p.x = xr.data_ptr();
-    p.w = (const int8_t*)w.data_ptr(); p.w_pitch = stride_or(w, 1, row_pitch(k)); p.w_scale = ws_c.data_ptr<float>();
+    p.batch = (int32_t)b; p.n_pix = n; p.x = xr.keep.data_ptr();
+    p.w = (const int8_t*)w.keep.data_ptr(); p.w_pitch = w.sn; p.w_scale = ws_c.data_ptr<float>();
     p.bias = bias ? b_c.data_ptr<float>() : nullptr;
     p.y = y.data_ptr();
     const size_t need = gnr_int8_linear_workspace_bytes(&p);
     TORCH_CHECK(need != 0, gnr_last_error());
     Tensor ws;
-    if (!rows8) ws = alloc_ws(need, dev);
-    check_rc(gnr_int8_linear(&p, rows8 ? nullptr : ws.data_ptr(), rows8 ? 0 : (size_t)ws.numel(), stream_of(dev)));
+    if (need > 256) ws = alloc_ws(need, dev);                  // 256: none is used
+    check_rc(gnr_int8_linear(&p, need > 256 ? ws.data_ptr() : nullptr, need > 256 ? (size_t)ws.numel() : 0, stream_of(dev)));
     return y;
 }
 

@@ -71,7 +71,7 @@ def _one_device(**ts):
 def _no_grad(what, *ts):
     if torch.is_grad_enabled():
         for t in ts:
-            if t is not None and torch.is_tensor(t) and t.requires_grad:
+            if getattr(t, "requires_grad", False):
                 raise RuntimeError("%s has no backward: call it under torch.no_grad() or on detached tensors" % what)
 
 

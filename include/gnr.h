@@ -387,7 +387,7 @@ typedef struct GnrInt8Problem {
 } GnrInt8Problem;
 #define GNR_INIT_INT8_PROBLEM { (uint32_t)sizeof(GnrInt8Problem) }
 
-size_t gnr_int8_linear_workspace_bytes(const GnrInt8Problem* p);     /* 0 + gnr_last_error() on bad input */
+size_t gnr_int8_linear_workspace_bytes(const GnrInt8Problem* p);     /* 0 + gnr_last_error() on bad input; 256: none is used, NULL will do */
 int gnr_int8_linear(const GnrInt8Problem* p, void* workspace, size_t ws_bytes, void* stream);
 
 /* The upsampler's forward (gnr_upsample_fwd) with its 1x1 convolutions in 8 bits: inference, no saved state.  Weights as

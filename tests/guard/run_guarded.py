@@ -22,6 +22,8 @@ Scenarios
   upsample      gnr_upsample_fwd / bwd over the shape generator of tests/diagnostics/fuzz_upsample.py + the cfg4 shape
                 (7 maps x 258 x 64 x 64 -> 512 x 512), each compared with the oracle
   aux           gnr_merge_fwd / bwd, gnr_resample, gnr_sample_zvals, the hierarchical pass, the view-direction option
+  int8          gnr_quantize_rows, gnr_read_rows, gnr_int8_linear and gnr_upsample_int8_fwd over random shapes, layouts and types, each compared
+                with a plain product of the same rows in 64 bits
   network_step  cfg4's whole-network training step (B = 2, 64 x 64 x 64 -> 512 x 512, loss, backward, Adam) x 2
 """
 import argparse
@@ -70,7 +72,8 @@ class Guard:
         from gazenerf_amd import _lib
         lib = _lib.load()
         for name in ("gnr_fwd", "gnr_fwd_bf16x3", "gnr_bwd", "gnr_bwd_bf16x3", "gnr_resample", "gnr_sample_zvals", "gnr_merge_fwd",
-                     "gnr_merge_bwd", "gnr_upsample_fwd", "gnr_upsample_bwd"):
+                     "gnr_merge_bwd", "gnr_upsample_fwd", "gnr_upsample_bwd", "gnr_quantize_rows", "gnr_read_rows", "gnr_int8_linear",
+                     "gnr_upsample_int8_fwd"):
             fn = getattr(lib, name)
 
             def make(fn=fn, name=name):
@@ -393,7 +396,89 @@ def sc_network_step(guard, args):
     return {"ok": ok, "cases": log}
 
 
-SCENARIOS = {"selftest": sc_selftest, "hot_path": sc_hot_path, "many_images": sc_many_images, "upsample": sc_upsample, "aux": sc_aux,
+def sc_int8(guard, args):
+    import math
+    import random
+
+    import torch
+    import gazenerf_amd as G
+    dev = torch.device("cuda:0")
+    rng = random.Random(args.seed)
+    g = torch.Generator().manual_seed(args.seed)
+    size = lambda lo, hi: int(round(math.exp(rng.uniform(math.log(lo), math.log(hi + 0.49)))))
+    types = (torch.float32, torch.bfloat16, torch.float16)
+    ok, log = True, []
+
+    def close(y, q, s, wq, b, leaky):
+        t = (q.double() @ wq.q.double().t()) * s.double().unsqueeze(-1) * wq.scale.double()
+        t = t + b.double() if b is not None else t
+        t = torch.where(t > 0, t, t * 0.2) if leaky else t
+        lim = torch.finfo(y.dtype).eps * t.abs() + 1e-5 * t.abs().max().clamp_min(1e-3)
+        return bool(((y.double() - t).abs() <= lim).all())
+
+    for case in range(args.cases):
+        dt, out = rng.choice(types), rng.choice(types)
+        k, o, p, b = size(1, 1100), size(1, 700), size(1, 700), rng.randint(1, 4)
+        if rng.random() < 0.15:
+            k, o, p, b = size(1024, 4100), size(256, 600), size(256, 300), 1
+        leaky, bias = rng.random() < 0.5, torch.randn(o, generator=g).to(dev) if rng.random() < 0.6 else None
+        wq = G.quantize_rows((torch.randn(o, k, generator=g) / k ** 0.5).to(dev))
+        x = torch.randn(b, k, p, generator=g).to(dt).to(dev)
+        n = b + rng.randint(0, 3)
+        q = torch.zeros(n, p, k, dtype=torch.int8, device=dev)             # rows behind each other: the last ends with its buffer
+        scale = torch.zeros(n, p, device=dev)
+        slots = torch.randperm(n, generator=g)[:b].to(dev)
+        G.write_featmaps(q, scale, slots, x)
+        new = guard.check("case %d after write_featmaps" % case)
+        r = G.quantize_rows(x, channels_first=True)
+        rr = G.quantize_rows(x.transpose(1, 2).contiguous())
+        new += guard.check("case %d after quantize_rows" % case)
+        far = torch.cat([slots, torch.tensor([-1, n, 1 << 40], device=dev)])
+        back = G.read_featmaps(q, scale, far, out)
+        new += guard.check("case %d after read_featmaps" % case)
+        good = torch.equal(q[slots], r.q) and torch.equal(r.q, rr.q) and torch.equal(r.scale, rr.scale) and torch.equal(scale[slots], r.scale)
+        good = good and torch.equal(back[:b], (r.q.float() * r.scale.unsqueeze(-1)).transpose(1, 2).to(out)) and bool((back[b] == 0).all()) \
+            and bool(torch.isnan(back[b + 1:]).all())
+        del back, rr
+        for cf in (False, True):
+            ys = [G.int8_linear(x if cf else x.transpose(1, 2).contiguous(), wq.q, wq.scale, bias, leaky=leaky, channels_first=cf, out_dtype=out)]
+            new += guard.check("case %d after int8_linear on values, cf %d" % (case, cf))
+            if not cf:
+                ys.append(G.int8_linear(x.transpose(1, 2).reshape(b * p, k), wq.q, wq.scale, bias, leaky=leaky, out_dtype=out).view(b, p, o))
+                ys.append(G.int8_linear(r.q[0, 0], wq.q, wq.scale, bias, x_scale=r.scale[0, 0], leaky=leaky, out_dtype=out).view(1, 1, o).expand(b, p, o))
+                new += guard.check("case %d after int8_linear on a list of rows" % case)
+            ys.append(G.int8_linear(r.q, wq.q, wq.scale, bias, x_scale=r.scale, leaky=leaky, channels_first=cf, out_dtype=out))
+            ys.append(G.int8_linear(q, wq.q, wq.scale, bias, x_scale=scale, slots=far, leaky=leaky, channels_first=cf, out_dtype=out))
+            new += guard.check("case %d after int8_linear on rows, cf %d" % (case, cf))
+            good = good and bool(torch.isnan(ys[-1][b + 1:]).all()) and finite(ys[-1][:b + 1])
+            ys[-1] = ys[-1][:b]
+            for i, y in enumerate(ys):
+                y = y.transpose(1, 2) if cf else y
+                if not cf and i == 2:
+                    good = good and close(y[:1, :1], r.q[:1, :1], r.scale[:1, :1], wq, bias, leaky)
+                else:
+                    good = good and close(y, r.q, r.scale, wq, bias, leaky)
+        good = good and new == 0
+        ok = ok and good
+        log.append("%s b %d p %d k %d o %d %s -> %s" % ("ok  " if good else "FAIL", b, p, k, o, dt, out))
+        print(log[-1], file=sys.stderr, flush=True)
+    for feat_nc, n_blocks, min_feat, S, B in ((6, 2, 4, 16, 2), (258, 1, 32, 16, 3), (129, 2, 32, 32, 1), (333, 1, 32, 16, 1), (64, 2, 32, 16, 2)):
+        net = G.NeuralRendererAMD(feat_nc=feat_nc, featmap_size=S, img_size=S << n_blocks, min_feat=min_feat, precision="int8", graph_inference=False).to(dev)
+        x = torch.randn(B, feat_nc, S, S, generator=g).to(dev)
+        cache = G.FeatureMapCache(B + 1, feat_nc, S * S, device=dev)
+        with torch.no_grad():
+            img = net(x)
+            cache.write(list(range(B)), x)
+            same = net.render_cached(cache, list(range(B)))
+        new = guard.check("after the 8-bit upsampler, %d channels" % feat_nc)
+        good = new == 0 and finite(img) and torch.equal(img, same)
+        ok = ok and good
+        log.append("%s upsampler feat_nc %d side %d blocks %d batch %d" % ("ok  " if good else "FAIL", feat_nc, S, n_blocks, B))
+        print(log[-1], file=sys.stderr, flush=True)
+    return {"ok": ok, "cases": log}
+
+
+SCENARIOS = {"int8": sc_int8, "selftest": sc_selftest, "hot_path": sc_hot_path, "many_images": sc_many_images, "upsample": sc_upsample, "aux": sc_aux,
              "network_step": sc_network_step}
 
 

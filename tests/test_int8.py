@@ -652,3 +652,14 @@ def test_two_bindings_agree(monkeypatch):
             G.write_featmaps(q, scale, slots.int(), maps)
     for i, (a, b) in enumerate(zip(*res)):
         assert a.shape == b.shape and a.dtype == b.dtype and torch.equal(a, b), i
+
+
+@gpu
+@pytest.mark.parametrize("binding, poison", [("ctypes", False), ("torch_ext", True)])
+def test_under_guard_bands(binding, poison):
+    """Random shapes with every device buffer fenced by 1 MiB of a known pattern (and, poisoned, full of 0xFF bytes: what lies between and
+    behind rows must not count, and no workspace is read before it is written)."""
+    from test_guard_bands import _guarded
+    d = _guarded("int8", "--binding", binding, "--cases", "25", "--seed", "7" if poison else "8", *(["--poison"] if poison else []))
+    assert d["ok"] and d["violations"] == 0, (d["report"], d["cases"])
+    assert d["calls_checked"] >= 25 * 6
