@@ -279,15 +279,18 @@ template <typename T, int LPX> static void quant_maps_lpx(const GnrRowsProblem& 
     switch (R) { GNR_MAPS(1); GNR_MAPS(2); GNR_MAPS(3); GNR_MAPS(4); }
 #undef GNR_MAPS
 }
-// 32 pixels a tile.  Threads: the fewest that keep a row in 4 quads of channels each (64 maps of 258 x 4096 in fp32: 78 us with 256 threads,
-// 90 with 512), twice that where the tiles do not fill the card (one map: 6.9 against 5.7 us).
+// 32 pixels a tile, 16 where an fp32 map would leave half the CUs without one (one map of 258 x 4096: 5.1 / 5.5 us).  Threads: the fewest that
+// keep a row in 4 quads of channels each (64 such maps: 78 us with 256 threads, 84 with 512), twice that while there are few of them (one
+// map: 6.8 / 5.5; five of 129 x 1369, bf16: 6.9 / 5.9).
 template <typename T> static void quant_maps(const GnrRowsProblem& p, hipStream_t st) {
     constexpr int LPX = 32 / Vec<T>::N;
     const int quads = (p.channels + 3) / 4;
+    const long tiles = (p.n_pix + 31) / 32 * p.batch;
     int nt = 64;
     while (nt < 1024 && quads > nt / LPX * 4) nt *= 2;
-    if ((p.n_pix + 31) / 32 * p.batch < 512 && nt < 1024 && quads > nt / LPX) nt *= 2;
-    quant_maps_lpx<T, LPX>(p, nt, st);
+    while (nt < 512 && tiles * nt < 131072 && quads > nt / LPX) nt *= 2;
+    if (sizeof(T) == 4 && tiles < 192 && nt > 64) quant_maps_lpx<T, 4>(p, nt, st);
+    else quant_maps_lpx<T, LPX>(p, nt, st);
 }
 
 template <typename T> static void quant_rows(const GnrRowsProblem& p, hipStream_t st) {
@@ -332,7 +335,11 @@ template <typename T, int LPX> static void read_maps_lpx(const GnrRowsProblem& p
     while (nt < 256 && (p.channels + 3) / 4 > nt / LPX) nt *= 2;
     hipLaunchKernelGGL((read_maps_kernel<T, LPX>), dim3(tiles * (unsigned)p.batch), dim3((unsigned)nt), sizeof(unsigned) * TP * ld, st, p, tiles, ld, step);
 }
-template <typename T> static void read_maps(const GnrRowsProblem& p, hipStream_t st) { read_maps_lpx<T, sizeof(T) == 4 ? 8 : 4>(p, st); }
+// 32 pixels a tile; 16 in fp32 while there are few (two maps of 258 x 4096: 5.5 / 6.6 us, 64: 52.7 / 51.4)
+template <typename T> static void read_maps(const GnrRowsProblem& p, hipStream_t st) {
+    if (sizeof(T) == 2 || (p.n_pix + 31) / 32 * p.batch < 2048) read_maps_lpx<T, 4>(p, st);
+    else read_maps_lpx<T, 8>(p, st);
+}
 
 }  // namespace gnr
 
