@@ -88,7 +88,7 @@ template <typename T> __device__ __forceinline__ float raw_value(const unsigned 
     else return (float)__builtin_bit_cast(T, (unsigned short)(w[v >> 1] >> 16 * (v & 1)));
 }
 
-// the row's scale and its reciprocal step from the largest abs_bits(); a row with an Inf / NaN: per = 0, scale = NaN
+// the row's scale and its reciprocal step from the bits of its largest |x|; a row with an Inf / NaN: per = 0, scale = NaN
 __device__ __forceinline__ void row_scale(unsigned a_bits, float& scale, float& per) {
     const bool bad = a_bits >= 0x7f800000u;
     const float a = __uint_as_float(a_bits > ROW_FLOOR_BITS ? a_bits : ROW_FLOOR_BITS);
@@ -119,6 +119,9 @@ __device__ __forceinline__ unsigned xcd_block(unsigned n) {
     return blockIdx.x < per * 8 ? (blockIdx.x & 7) * per + (blockIdx.x >> 3) : blockIdx.x;
 }
 
-int check_rows(const GnrRowsProblem* p, const char* what);
+// A grid counts its threads in 32 bits; a larger one is cut off without an error
+inline int check_grid(const char* what, long blocks, long threads) {
+    return blocks * threads < (1L << 32) ? 0 : fail("%s: %ld workgroups of %ld threads exceed one launch", what, blocks, threads);
+}
 int launch_quantize(const GnrRowsProblem& p, hipStream_t st);        // defined in gnr_quant.hip; 0 == enqueued
 }  // namespace gnr

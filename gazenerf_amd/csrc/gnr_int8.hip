@@ -591,6 +591,7 @@ static int check_int8(const GnrInt8Problem* p) {
     if (p->y_type != GNR_F32 && p->y_type != GNR_BF16 && p->y_type != GNR_F16) return fail("gnr_int8_linear: unknown y_type %d", p->y_type);
     if (p->batch < 0 || p->n_pix < 0) return fail("gnr_int8_linear: batch and n_pix must be >= 0");
     if (p->k < 1 || p->o < 1) return fail("gnr_int8_linear: k and o must be >= 1 (got %d, %d)", p->k, p->o);
+    if (p->o > 1 << 27) return fail("gnr_int8_linear: o = %d exceeds 2^27", p->o);
     if (p->k > GNR_INT8_MAX_K) return fail("gnr_int8_linear: k = %d exceeds %d: the 32-bit sum could overflow", p->k, GNR_INT8_MAX_K);
     if (p->x_channels_first && rows8) return fail("gnr_int8_linear: 8-bit rows have their channels last");
     if (p->slots && !rows8) return fail("gnr_int8_linear: slots name rows of a cache, x must be 8-bit rows");
@@ -633,7 +634,7 @@ static int int8_fuse(const GnrInt8Problem* p) {
     while (cf && nmt > 1 && p->k > 32 * vec * 4 / nmt) nmt /= 2;               // maps: 4 quads of channels a thread
     if (cf && p->k > 32 * vec * 4 / nmt) return FUSE_NONE;
     const long groups = cf ? p->batch * ((p->n_pix + 32 * nmt - 1) / (32 * nmt)) : (N + 32 * nmt - 1) / (32 * nmt), parts = fused_parts(p->o, nmt, &span);
-    if (groups * parts >= (1L << 31)) return FUSE_NONE;
+    if (groups * parts * 256 >= (1L << 32)) return FUSE_NONE;                  // check_grid
     return p->o <= 128 || groups * parts <= 256 ? nmt : FUSE_NONE;
 }
 
@@ -654,7 +655,7 @@ template <typename T, bool CF, int WM, int WN, int TM, int TN, int NST = 4> stat
     typedef TileShape<WM, WN, TM, TN, NST> S;
     const long M = CF ? a.P : a.O, N = CF ? a.O : a.N;
     const long tm = (M + S::BM - 1) / S::BM, tn = (N + S::BN - 1) / S::BN, tiles = tm * tn * (CF ? batch : 1);
-    if (tiles >= (1L << 31)) return fail("gnr_int8_linear: %ld tiles exceed one launch", tiles);
+    if (check_grid("gnr_int8_linear", tiles, S::NT)) return 1;
     const int stages = (a.K + 63) / 64 < NST ? (a.K + 63) / 64 : NST, ring = stages * S::STAGE;
     hipLaunchKernelGGL((int8_tile_kernel<T, CF, WM, WN, TM, TN, NST>), dim3((unsigned)tiles), dim3(S::NT), ring > S::TURN ? ring : S::TURN, st, a,
                        (unsigned)tm, (unsigned)tn);

@@ -117,10 +117,10 @@ __global__ __launch_bounds__(1024) void quant_maps_kernel(const GnrRowsProblem p
 // rows [N][C] -> rows: L lanes share a row and keep J pieces of 16 bytes each; rows wider than L J V are read twice
 // ---------------------------------------------------------------------------------------------
 template <typename T, int L, int J>
-__global__ __launch_bounds__(256) void quant_rows_kernel(const GnrRowsProblem p, long total) {
+__global__ __launch_bounds__(256) void quant_rows_kernel(const GnrRowsProblem p, long first, long total) {
     constexpr int V = Vec<T>::N;
     const int lane = (int)threadIdx.x % L;
-    const long n = (long)blockIdx.x * (256 / L) + (int)threadIdx.x / L;
+    const long n = first + (long)blockIdx.x * (256 / L) + (int)threadIdx.x / L;
     const bool ok = n < total;
     const unsigned b = ok ? (unsigned)n / (unsigned)p.n_pix : 0, pix = ok ? (unsigned)n - b * (unsigned)p.n_pix : 0;     // rows: at most 2^31
     const T* x = (const T*)p.x + b * p.x_batch + pix * p.x_stride;
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(256) void read_maps_kernel(const GnrRowsProblem p, 
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
-int check_rows(const GnrRowsProblem* p, const char* what) {
+static int check_rows(const GnrRowsProblem* p, const char* what) {
     if (!p) return fail("%s: problem is NULL", what);
     if (p->struct_size != sizeof(GnrRowsProblem))
         return fail("%s: GnrRowsProblem.struct_size is %u but this libgnr.so (ABI %d) has sizeof = %zu: the caller was built "
@@ -257,7 +257,7 @@ int check_rows(const GnrRowsProblem* p, const char* what) {
                     sizeof(GnrRowsProblem));
     if (p->dtype != GNR_F32 && p->dtype != GNR_BF16 && p->dtype != GNR_F16) return fail("%s: unknown dtype %d", what, p->dtype);
     if (p->batch < 0 || p->n_pix < 0) return fail("%s: batch and n_pix must be >= 0", what);
-    if (p->channels < 1) return fail("%s: channels must be >= 1 (got %d)", what, p->channels);
+    if (p->channels < 1 || p->channels > 1 << 30) return fail("%s: channels must be 1 .. 2^30 (got %d)", what, p->channels);
     if (p->batch == 0 || p->n_pix == 0) return 0;
     if (p->n_pix > (1LL << 31) / p->batch) return fail("%s: %d x %lld rows exceed 2^31", what, p->batch, (long long)p->n_pix);
     if (!p->x || !p->q || !p->scale) return fail("%s: NULL pointer", what);
@@ -267,37 +267,45 @@ int check_rows(const GnrRowsProblem* p, const char* what) {
     return 0;
 }
 
-template <typename T, int LPX> static void quant_maps_lpx(const GnrRowsProblem& p, int nt, hipStream_t st) {
+template <typename T, int LPX> static int quant_maps_lpx(const GnrRowsProblem& p, int nt, hipStream_t st) {
     constexpr int TP = LPX * Vec<T>::N;
     const unsigned tiles = (unsigned)((p.n_pix + TP - 1) / TP);
     const int quads = (p.channels + 3) / 4, G = nt / LPX;
     const int R = quads >= 4 * G ? 4 : (quads + G - 1) / G;
     const int words = quads < G * R ? quads : G * R, ld = (words + 15) / 16 * 16 + 4;
     const size_t lds = sizeof(unsigned) * ((size_t)TP * ld + (size_t)nt / 64 * LPX * 4);
+    if (check_grid("gnr_quantize_rows", (long)tiles * p.batch, nt)) return 1;
     const dim3 grid(tiles * (unsigned)p.batch), block((unsigned)nt);
 #define GNR_MAPS(RR) case RR: hipLaunchKernelGGL((quant_maps_kernel<T, LPX, RR>), grid, block, lds, st, p, tiles, ld); break
     switch (R) { GNR_MAPS(1); GNR_MAPS(2); GNR_MAPS(3); GNR_MAPS(4); }
 #undef GNR_MAPS
+    return 0;
 }
 // 32 pixels a tile, 16 where an fp32 map would leave half the CUs without one (one map of 258 x 4096: 5.1 / 5.5 us).  Threads: the fewest that
 // keep a row in 4 quads of channels each (64 such maps: 78 us with 256 threads, 84 with 512), twice that while there are few of them (one
 // map: 6.8 / 5.5; five of 129 x 1369, bf16: 6.9 / 5.9).
-template <typename T> static void quant_maps(const GnrRowsProblem& p, hipStream_t st) {
+template <typename T> static int quant_maps(const GnrRowsProblem& p, hipStream_t st) {
     constexpr int LPX = 32 / Vec<T>::N;
     const int quads = (p.channels + 3) / 4;
     const long tiles = (p.n_pix + 31) / 32 * p.batch;
     int nt = 64;
     while (nt < 1024 && quads > nt / LPX * 4) nt *= 2;
     while (nt < 512 && tiles * nt < 131072 && quads > nt / LPX) nt *= 2;
-    if (sizeof(T) == 4 && tiles < 192 && nt > 64) quant_maps_lpx<T, 4>(p, nt, st);
-    else quant_maps_lpx<T, LPX>(p, nt, st);
+    if (sizeof(T) == 4 && tiles < 192 && nt > 64) return quant_maps_lpx<T, 4>(p, nt, st);
+    return quant_maps_lpx<T, LPX>(p, nt, st);
 }
 
-template <typename T> static void quant_rows(const GnrRowsProblem& p, hipStream_t st) {
+template <typename T, int L, int J> static void quant_rows_lj(const GnrRowsProblem& p, hipStream_t st) {
+    const long total = (long)p.batch * p.n_pix, most = (1L << 27) / L * 16;    // a launch's threads: 2^31
+    for (long first = 0; first < total; first += most) {
+        const long n = total - first < most ? total - first : most;
+        hipLaunchKernelGGL((quant_rows_kernel<T, L, J>), dim3((unsigned)((n + 256 / L - 1) / (256 / L))), dim3(256), 0, st, p, first, total);
+    }
+}
+template <typename T> static int quant_rows(const GnrRowsProblem& p, hipStream_t st) {
     constexpr int V = Vec<T>::N;
-    const long total = (long)p.batch * p.n_pix;
     const int C = p.channels;
-#define GNR_ROWS(L, J) hipLaunchKernelGGL((quant_rows_kernel<T, L, J>), dim3((unsigned)((total + 256 / L - 1) / (256 / L))), dim3(256), 0, st, p, total)
+#define GNR_ROWS(L, J) quant_rows_lj<T, L, J>(p, st)
     switch ((C + 16 * V - 1) / (16 * V)) {                     // 16 lanes a row while eight pieces a lane hold it
         case 1: GNR_ROWS(16, 1); break;
         case 2: GNR_ROWS(16, 2); break;
@@ -311,34 +319,32 @@ template <typename T> static void quant_rows(const GnrRowsProblem& p, hipStream_
             else GNR_ROWS(64, 8);
     }
 #undef GNR_ROWS
+    return 0;
 }
 
 int launch_quantize(const GnrRowsProblem& p, hipStream_t st) {
-    if (p.channels_first) {
-        if (p.dtype == GNR_F32) quant_maps<float>(p, st);
-        else if (p.dtype == GNR_BF16) quant_maps<__bf16>(p, st);
-        else quant_maps<_Float16>(p, st);
-    } else {
-        if (p.dtype == GNR_F32) quant_rows<float>(p, st);
-        else if (p.dtype == GNR_BF16) quant_rows<__bf16>(p, st);
-        else quant_rows<_Float16>(p, st);
-    }
+    int rc;
+    if (p.channels_first) rc = p.dtype == GNR_F32 ? quant_maps<float>(p, st) : p.dtype == GNR_BF16 ? quant_maps<__bf16>(p, st) : quant_maps<_Float16>(p, st);
+    else rc = p.dtype == GNR_F32 ? quant_rows<float>(p, st) : p.dtype == GNR_BF16 ? quant_rows<__bf16>(p, st) : quant_rows<_Float16>(p, st);
+    if (rc) return 1;
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : fail("gnr_quantize_rows: launch failed: %s", hipGetErrorString(e));
 }
 
-template <typename T, int LPX> static void read_maps_lpx(const GnrRowsProblem& p, hipStream_t st) {
+template <typename T, int LPX> static int read_maps_lpx(const GnrRowsProblem& p, hipStream_t st) {
     constexpr int TP = LPX * Vec<T>::N;
     const unsigned tiles = (unsigned)((p.n_pix + TP - 1) / TP);
     const int step = p.channels < 1920 ? p.channels : 1920, ld = (step + 63) / 64 * 16 + 4;
     int nt = 64;                                               // a quad of channels a thread and turn: no more threads than quads
     while (nt < 256 && (p.channels + 3) / 4 > nt / LPX) nt *= 2;
+    if (check_grid("gnr_read_rows", (long)tiles * p.batch, nt)) return 1;
     hipLaunchKernelGGL((read_maps_kernel<T, LPX>), dim3(tiles * (unsigned)p.batch), dim3((unsigned)nt), sizeof(unsigned) * TP * ld, st, p, tiles, ld, step);
+    return 0;
 }
 // 32 pixels a tile; 16 in fp32 while there are few (two maps of 258 x 4096: 5.5 / 6.6 us, 64: 52.7 / 51.4)
-template <typename T> static void read_maps(const GnrRowsProblem& p, hipStream_t st) {
-    if (sizeof(T) == 2 || (p.n_pix + 31) / 32 * p.batch < 2048) read_maps_lpx<T, 4>(p, st);
-    else read_maps_lpx<T, 8>(p, st);
+template <typename T> static int read_maps(const GnrRowsProblem& p, hipStream_t st) {
+    if (sizeof(T) == 2 || (p.n_pix + 31) / 32 * p.batch < 2048) return read_maps_lpx<T, 4>(p, st);
+    return read_maps_lpx<T, 8>(p, st);
 }
 
 }  // namespace gnr
@@ -359,9 +365,7 @@ int gnr_read_rows(const GnrRowsProblem* p, void* stream) {
     if (!p->channels_first) return fail("gnr_read_rows: reads into channels-first maps only");
     if (p->batch == 0 || p->n_pix == 0) return 0;
     hipStream_t st = (hipStream_t)stream;
-    if (p->dtype == GNR_F32) read_maps<float>(*p, st);
-    else if (p->dtype == GNR_BF16) read_maps<__bf16>(*p, st);
-    else read_maps<_Float16>(*p, st);
+    if (p->dtype == GNR_F32 ? read_maps<float>(*p, st) : p->dtype == GNR_BF16 ? read_maps<__bf16>(*p, st) : read_maps<_Float16>(*p, st)) return 1;
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : fail("gnr_read_rows: launch failed: %s", hipGetErrorString(e));
 }

@@ -428,7 +428,7 @@ Tensor int8_linear(const Tensor& x, const Tensor& w_q, const Tensor& w_scale, co
     check_on(w_q, "w_q", at::kChar, 2, dev);
     check_on(w_scale, "w_scale", at::kFloat, 1, dev);
     const int64_t o = w_q.size(0), k = w_q.size(1);
-    TORCH_CHECK(o >= 1 && k >= 1 && o <= INT32_MAX && k <= GNR_INT8_MAX_K, "w_q has a shape the product cannot take: ", w_q.sizes());
+    TORCH_CHECK(o >= 1 && k >= 1 && o <= 1 << 27 && k <= GNR_INT8_MAX_K, "w_q has a shape the product cannot take: ", w_q.sizes());
     TORCH_CHECK(w_scale.size(0) == o, "w_scale must have shape [", o, "], got ", w_scale.sizes());
     GnrInt8Problem p = GNR_INIT_INT8_PROBLEM;
     p.x_type = rows8 ? GNR_I8 : type_id(x.scalar_type(), "x");

@@ -21,6 +21,7 @@ device.  There is no backward: a call on inputs that would need a gradient is re
 from __future__ import annotations
 
 import ctypes as C
+import operator
 from typing import NamedTuple, Optional
 
 import torch
@@ -106,6 +107,8 @@ def _check_linear(x, w_q, w_scale, bias, x_scale, slots, channels_first, out_dty
     o, k = w_q.shape
     if o < 1 or k < 1:
         raise ValueError("w_q is empty: %s" % (tuple(w_q.shape),))
+    if o > 1 << 27:
+        raise ValueError("w_q has %d outputs, at most 2^27 fit one launch" % o)
     if k > _lib.INT8_MAX_K:
         raise ValueError("w_q has %d channels, at most %d are summed exactly in 32 bits" % (k, _lib.INT8_MAX_K))
     if w_scale.shape[0] != o:
@@ -268,7 +271,7 @@ def write_featmaps(q, scale, slots, maps) -> None:
 
     ``slots``: int64 [B] on the device, not read by the host.  A negative slot is padding and a slot >= n a mistake: neither is
     written.  Of several maps with the same slot the last one stays.  Every other byte of the cache is left as it was."""
-    _no_grad("write_featmaps", maps)
+    _no_grad("write_featmaps", maps, scale)
     ext = _torch_ext.active()
     if ext is not None:
         try:
@@ -292,6 +295,7 @@ def _check_write(q, scale, slots, maps):
 
 def read_featmaps(q, scale, slots, out_dtype=torch.float32):
     """slots int64 [B] of the cache -> maps [B, C, P].  A negative slot reads as zeros, a slot >= n as NaN."""
+    _no_grad("read_featmaps", scale)
     ext = _torch_ext.active()
     if ext is not None and out_dtype in _FLOATS:
         try:
@@ -405,7 +409,7 @@ class FeatureMapCache:
     def slots(self, slots) -> torch.Tensor:
         if torch.is_tensor(slots):
             return slots
-        slots = [slots] if isinstance(slots, int) else [int(s) for s in slots]
+        slots = [operator.index(s) for s in ([slots] if hasattr(slots, "__index__") else slots)]
         for s in slots:
             if s >= self.n_slots:
                 raise IndexError("slot %d of a cache of %d" % (s, self.n_slots))

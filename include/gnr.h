@@ -369,7 +369,7 @@ typedef struct GnrInt8Problem {
     int32_t leaky;              /* LeakyReLU(0.2) behind the bias                                                */
     int32_t x_channels_first;   /* floating x only: maps instead of rows (GnrRowsProblem)                        */
     int32_t y_channels_first;   /* y [batch][o][n_pix] instead of [batch][n_pix][o]; contiguous                  */
-    int32_t batch, k, o, reserved;
+    int32_t batch, k, o, reserved;           /* o <= 2^27 */
     int64_t n_pix;
     const void* x;
     int64_t x_batch, x_stride;  /* strides as in GnrRowsProblem, in elements.  GNR_I8: x 16-byte aligned, both multiples of 16,

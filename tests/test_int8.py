@@ -8,6 +8,7 @@ relative to |s| + |bias| -- and once to the output type (eps / 2; below the fp16
 import ctypes as C
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -173,6 +174,11 @@ def test_no_backward(lib_built):
         G.quantize_rows(x)
     with pytest.raises(RuntimeError, match="no backward"):
         G.write_featmaps(torch.zeros(1, 3, 16, dtype=torch.int8), torch.zeros(1, 3), torch.zeros(1, dtype=torch.int64), x.t()[None])
+    cache = torch.zeros(1, 3, 16, dtype=torch.int8), torch.ones(1, 3, requires_grad=True), torch.zeros(1, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="no backward"):
+        G.write_featmaps(*cache, torch.zeros(1, 16, 3))
+    with pytest.raises(RuntimeError, match="no backward"):
+        G.read_featmaps(*cache)
     with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA/ROCm"):       # no gradient wanted: the next check speaks
         G.int8_linear(x, w, torch.ones(5))
 
@@ -198,6 +204,8 @@ def test_c_entries_refuse(lib_built):
                          (dict(n_pix=1 << 31), "2^31"), (dict(channels_first=0), "channels-first")):
             assert fn(C.byref(rows(**kw)), None) != 0, kw
             assert word in lib.gnr_last_error().decode(), (kw, lib.gnr_last_error())
+        huge = dict(dtype=1, batch=1, n_pix=1 << 31, channels=4096, q_pitch=4096, slots=None, n_slots=0)      # more threads than a grid counts
+        assert fn(C.byref(rows(**huge)), None) != 0 and "exceed one launch" in lib.gnr_last_error().decode()
         assert fn(C.byref(rows(batch=0)), None) == 0 and fn(C.byref(rows(n_pix=0)), None) == 0      # an empty call
 
     def lin(**kw):
@@ -210,7 +218,7 @@ def test_c_entries_refuse(lib_built):
         return p
 
     bad = ((dict(struct_size=8), "struct_size"), (dict(x_type=4), "x_type"), (dict(y_type=3), "y_type"), (dict(batch=-1), "batch"), (dict(k=0), "k and o"),
-           (dict(o=0), "k and o"), (dict(k=131072, w_pitch=131072), "exceeds"), (dict(x_channels_first=1), "channels last"),
+           (dict(o=0), "k and o"), (dict(k=131072, w_pitch=131072), "exceeds"), (dict(o=(1 << 27) + 1), "exceeds"), (dict(x_channels_first=1), "channels last"),
            (dict(x_type=0), "slots"), (dict(n_slots=0), "n_slots"), (dict(n_pix=1 << 31), "2^31"), (dict(x=None), "NULL"), (dict(w=None), "NULL"),
            (dict(y=None), "NULL"), (dict(w_scale=None), "NULL"), (dict(x_scale=None), "x_scale"), (dict(w=4097), "16-byte"), (dict(w_pitch=24), "16-byte"),
            (dict(w_pitch=16), "16-byte"), (dict(x=4100), "16-byte"), (dict(x_stride=40), "16-byte"), (dict(x_stride=16), "16-byte"),
@@ -221,6 +229,8 @@ def test_c_entries_refuse(lib_built):
         assert lib.gnr_int8_linear_workspace_bytes(C.byref(lin(**kw))) == 0, kw
     assert lib.gnr_int8_linear(None, None, 0, None) != 0
     assert lib.gnr_int8_linear(C.byref(lin(batch=0)), None, 0, None) == 0
+    assert lib.gnr_int8_linear(C.byref(lin(batch=1 << 25, n_pix=33, y_channels_first=1)), None, 0, None) != 0
+    assert "exceed one launch" in lib.gnr_last_error().decode()
     flt = dict(x_type=0, slots=None, n_slots=0)
     need = lib.gnr_int8_linear_workspace_bytes(C.byref(lin(**flt)))
     assert need >= 16 * 32 + 16 * 4                                     # the rows on their pitch and their scales
@@ -377,6 +387,21 @@ def test_cache_strides():
 
 
 @gpu
+def test_quantize_more_rows_than_one_launch():
+    """A grid counts its threads in 32 bits: 16 lanes a row reach that at 2^28 rows, launches end at 2^27."""
+    n, at = (1 << 28) + 33, 1 << 27
+    x = torch.full((n, 1), 1.5, dtype=torch.bfloat16, device=DEV)
+    probe = torch.tensor([0, 1, at - 1, at, at + 1, 2 * at - 1, 2 * at, n - 2, n - 1], device=DEV)
+    x[probe] = torch.tensor([[-1.0], [0.0], [2.5], [-3.25], [1e-20], [-7.0], [0.5], [1e20], [-0.125]], dtype=torch.bfloat16, device=DEV)
+    q, scale = G.quantize_rows(x)
+    want_q, want_s = ref_rows(x[probe])
+    assert torch.equal(q[probe].cpu().double(), want_q) and torch.equal(scale[probe].cpu(), want_s)
+    rest = torch.ones(n, dtype=torch.bool, device=DEV)
+    rest[probe] = False
+    assert bool((scale[rest] == ref_rows(torch.tensor([1.5]))[1].item()).all()) and bool((q[:, 0][rest] == 127).all())
+
+
+@gpu
 def test_cache_offsets_beyond_32_bits():
     """Slots whose bytes lie behind 2^32."""
     c, p, n = 1024, 4096, 1100
@@ -408,6 +433,7 @@ def test_feature_map_cache():
     err = (cache.read([3, 1]).cpu().double() - maps.flatten(2).cpu().double()).abs()
     step = want_s.double().unsqueeze(1)
     assert bool((err <= step * (0.5 + 127 * 2.0 ** -22)).all())
+    assert torch.equal(cache.read(np.int64(3)), cache.read([np.int32(3)]))
     w, b = weights(17, 30, 1)
     wq = G.quantize_rows(w.to(DEV))
     ref, bound = ref_linear(want_q, want_s, wq.q, wq.scale, b, True)
