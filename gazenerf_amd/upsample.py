@@ -260,13 +260,12 @@ class NeuralRendererAMD(nn.Module):
     def __init__(self, bg_type="white", feat_nc=258, out_dim=3, final_actvn=True, min_feat=32, featmap_size=64,
                  img_size=512, graph_inference=True, precision="fp32", **kwargs):
         super().__init__()
-        from .upsample8 import GraphedUpsample8, Int8Weights
+        from .upsample8 import Int8Renderers
         # precision="int8": inference in 8 bits (gazenerf_amd.upsample8); calls that need gradients are refused
         if precision not in ("fp32", "int8"):
             raise ValueError("precision must be 'fp32' or 'int8'")
         self.precision = precision
-        self._int8_weights = Int8Weights()
-        self._graphed8 = GraphedUpsample8(self._int8_weights)
+        self._int8 = Int8Renderers()
         # graph_inference: under torch.no_grad() the forward is replayed from a HIP graph (GraphedUpsample) -- the
         # reference's render loops call the network one image at a time, where launch gaps were a fifth of the call
         self.graph_inference = bool(graph_inference)
@@ -295,9 +294,11 @@ class NeuralRendererAMD(nn.Module):
         from .upsample8 import neural_render_int8
         params = {k: v for k, v in self.named_parameters() if k != "bg_featmap"}
         dev = x if x is not None else cache.q
-        if self.graph_inference and not torch.is_grad_enabled() and dev.is_cuda and not torch.cuda.is_current_stream_capturing():
-            return self._graphed8(params, self.n_blocks, self.min_feat, self.final_actvn, x, cache, slots)
-        return neural_render_int8(x, params, self.n_blocks, self.min_feat, self.final_actvn, self._int8_weights, cache, slots)
+        capturing = dev.is_cuda and torch.cuda.is_current_stream_capturing()
+        if self.graph_inference and not torch.is_grad_enabled() and dev.is_cuda and not capturing:
+            return self._int8(dev.device)(params, self.n_blocks, self.min_feat, self.final_actvn, x, cache, slots)
+        weights = None if capturing else self._int8(dev.device).weights
+        return neural_render_int8(x, params, self.n_blocks, self.min_feat, self.final_actvn, weights, cache, slots)
 
     def render_cached(self, cache, slots):
         """Images [B, 3, ..] of the feature maps in ``slots`` of a ``FeatureMapCache`` (an int, a sequence or an int64 tensor on its device), in
@@ -318,14 +319,19 @@ class NeuralRendererAMD(nn.Module):
 
     def _apply(self, fn, *args, **kw):          # .to() / .cuda() / .half(): parameters move, captured graphs are stale
         self._graphed.clear()
-        self._graphed8.clear()
-        self._int8_weights.clear()
+        self._int8.clear()
         return super()._apply(fn, *args, **kw)
 
     def train(self, mode: bool = True):         # the quantised weights would miss an in-place write through ``.data``
-        self._int8_weights.seen = None
+        self._int8.look_again()
         return super().train(mode)
 
     def load_state_dict(self, *args, **kwargs):
-        self._int8_weights.seen = None
+        self._int8.look_again()
         return super().load_state_dict(*args, **kwargs)
+
+    def __setstate__(self, state):              # a module pickled before there was a precision
+        from .upsample8 import Int8Renderers
+        super().__setstate__(state)
+        self.__dict__.setdefault("precision", "fp32")
+        self.__dict__.setdefault("_int8", Int8Renderers())

@@ -7,7 +7,6 @@ reads as they are; both give the same image bit for bit.  There is no backward.
 """
 from __future__ import annotations
 
-import copy
 import ctypes as C
 from typing import Dict, Optional
 
@@ -23,8 +22,8 @@ _CONVS = (("up1", "feat_upsample_list.%d.layer_1"), ("up2", "feat_upsample_list.
 class Int8Weights:
     """The renderer's convolution weights as 8-bit rows, quantised once and again when a parameter changed: another tensor, a
     higher ``_version`` (torch counts every in-place write) or another ``data_ptr()``.  An in-place write through ``.data`` is invisible to
-    all three: call ``clear()`` after one.  The buffers stay where they are while shapes and device do, so captured graphs that read
-    them see the new values.  One per module and HIP stream."""
+    all three, and so is one by a replayed graph: call ``clear()`` after one.  The buffers stay where they are while shapes and device do,
+    so captured graphs that read them see the new values.  One per module and HIP stream (``Int8Renderers``)."""
 
     def __init__(self):
         self.rows: Dict[str, int8.QuantizedRows] = {}
@@ -34,19 +33,11 @@ class Int8Weights:
     def clear(self):
         self.__init__()
 
-    def __deepcopy__(self, memo):
-        return Int8Weights()
-
-    def __getstate__(self):
-        return {}
-
-    def __setstate__(self, state):
-        self.__init__()
-
     def refresh(self, params: Dict[str, torch.Tensor], n_blocks: int) -> None:
         names = [name % i for i in range(n_blocks) for _, name in _CONVS]
         flat = [params[n + ".weight"] for n in names]
-        if self.seen is not None and len(self.seen) == len(flat) and all(
+        counted = not any(t.is_inference() for t in flat)       # torch counts no writes to tensors made in inference mode
+        if counted and self.seen is not None and len(self.seen) == len(flat) and all(
                 a is t and v == t._version and d == t.data_ptr() for (a, v, d), t in zip(self.seen, flat)):
             return
         self.seen = None                                        # a call that raises half-way leaves nothing that looks current
@@ -57,7 +48,8 @@ class Int8Weights:
                 q = int8.empty_rows(*t2.shape, device=t2.device)
                 old = self.rows[n] = int8.QuantizedRows(q, torch.empty(t2.shape[0], dtype=torch.float32, device=t2.device))
             int8.quantize_rows_into(t2, old.q, old.scale)
-        self.seen = [(t, t._version, t.data_ptr()) for t in flat]
+        if counted:
+            self.seen = [(t, t._version, t.data_ptr()) for t in flat]
         self.quantised += 1
 
     def fill(self, s: "_lib.GnrUpsampleInt8", n_blocks: int):
@@ -143,9 +135,13 @@ class _Call:
 def neural_render_int8(x, params: Dict[str, torch.Tensor], n_blocks: int = 3, min_feat: int = 32, final_actvn: bool = True,
                        weights: Optional[Int8Weights] = None, cache=None, slots=None):
     """``neural_render`` in 8 bits: x [B, feat_nc, S, S] -- or x None with a ``FeatureMapCache`` and int64 ``slots`` [B] on its device --
-    -> image [B, 3, S*2^n, S*2^n].  ``weights`` keeps the quantised weights from call to call.  Inference only."""
+    -> image [B, 3, S*2^n, S*2^n].  ``weights`` keeps the quantised weights from call to call; a call that is being captured quantises them
+    in the graph instead, so that a replay follows its parameters.  Inference only."""
     int8._no_grad("neural_render_int8", x, *params.values())
-    return _Call(params, weights if weights is not None else Int8Weights(), int(n_blocks), int(min_feat), bool(final_actvn), x, cache, slots)()
+    dev = x if x is not None else getattr(cache, "q", None)
+    if weights is None or (getattr(dev, "is_cuda", False) and torch.cuda.is_current_stream_capturing()):
+        weights = Int8Weights()
+    return _Call(params, weights, int(n_blocks), int(min_feat), bool(final_actvn), x, cache, slots)()
 
 
 class GraphedUpsample8:
@@ -160,16 +156,6 @@ class GraphedUpsample8:
 
     def clear(self):
         self.entries.clear()
-
-    # the entries hold CUDAGraph objects and structs of device pointers: a copy starts without them
-    def __deepcopy__(self, memo):
-        return GraphedUpsample8(copy.deepcopy(self.weights, memo), self.max_entries)
-
-    def __getstate__(self):
-        return {"weights": self.weights, "max_entries": self.max_entries}
-
-    def __setstate__(self, state):
-        self.__init__(state["weights"], state["max_entries"])
 
     def __call__(self, params, n_blocks, min_feat, final_actvn, x=None, cache=None, slots=None):
         self.weights.refresh(params, n_blocks)
@@ -213,3 +199,39 @@ class GraphedUpsample8:
                 call()
         self.captures += 1
         return graph, static, call
+
+
+class Int8Renderers:
+    """A ``GraphedUpsample8`` (with its ``Int8Weights``) per HIP stream: what two streams run at once shares no buffer.  The
+    ``max_streams`` used last are kept.  A copy starts empty: graphs and structs of device pointers are not copied."""
+
+    def __init__(self, max_streams: int = 4):
+        self.max_streams = max_streams
+        self.streams = {}
+
+    def __call__(self, dev) -> GraphedUpsample8:
+        key = torch.cuda.current_stream(dev).cuda_stream if dev.type == "cuda" else None
+        r = self.streams.pop((dev, key), None)
+        if r is None:
+            r = GraphedUpsample8(Int8Weights())
+            while len(self.streams) >= self.max_streams:
+                self.streams.pop(next(iter(self.streams)))
+        self.streams[dev, key] = r
+        return r
+
+    def look_again(self):
+        """The next call on each stream quantises its weights again."""
+        for r in self.streams.values():
+            r.weights.seen = None
+
+    def clear(self):
+        self.streams.clear()
+
+    def __deepcopy__(self, memo):
+        return Int8Renderers(self.max_streams)
+
+    def __getstate__(self):
+        return {"max_streams": self.max_streams}
+
+    def __setstate__(self, state):
+        self.__init__(state["max_streams"])

@@ -7,6 +7,7 @@ magnitudes), the upsampling of the running image (bilinear and blur: fewer than 
 the sigmoid (slope at most 1/4, expf and the quotient within 4 u of a value below 1)."""
 import copy
 import ctypes as C
+import pickle
 
 import pytest
 import torch
@@ -137,9 +138,9 @@ def test_image_from_cached_rows():
     assert torch.equal(odd.nan_to_num(), img.nan_to_num())
 
 
-def small_renderer(**kw):
+def small_renderer(device=DEV, **kw):
     torch.manual_seed(0)
-    return G.NeuralRendererAMD(feat_nc=36, featmap_size=16, img_size=64, min_feat=8, **kw).to(DEV)
+    return G.NeuralRendererAMD(feat_nc=36, featmap_size=16, img_size=64, min_feat=8, **kw).to(device)
 
 
 @gpu
@@ -152,13 +153,14 @@ def test_module_replays_and_follows_its_parameters():
     with torch.no_grad():
         for x in xs:
             assert torch.equal(net(x), eager(x))
-        assert net._graphed8.captures == 2 and net._graphed8.replays == 5 and net._int8_weights.quantised == 1
+        graphed = net._int8(torch.device(DEV, torch.cuda.current_device()))
+        assert graphed.captures == 2 and graphed.replays == 5 and graphed.weights.quantised == 1
         before = net(xs[0])
         net.feat_layers[0].weight.mul_(1.5)                                     # counted by torch
         net.feat_2_rgb_list[1].bias.add_(0.25)                                  # read in place by the graph
         for x in xs[:3]:
             assert torch.equal(net(x), eager(x))
-        assert not torch.equal(net(xs[0]), before) and net._int8_weights.quantised == 2 and net._graphed8.captures == 2
+        assert not torch.equal(net(xs[0]), before) and graphed.weights.quantised == 2 and graphed.captures == 2
         state = {k: v * 0.5 for k, v in net.state_dict().items()}
         net.load_state_dict(state)
         assert torch.equal(net(xs[0]), eager(xs[0]))
@@ -166,9 +168,75 @@ def test_module_replays_and_follows_its_parameters():
         net.eval()
         assert torch.equal(net(xs[1]), eager(xs[1]))
         twin = copy.deepcopy(net)
-        assert torch.equal(twin(xs[0]), net(xs[0])) and twin._graphed8 is not net._graphed8
+        assert torch.equal(twin(xs[0]), net(xs[0])) and twin._int8 is not net._int8
     with torch.inference_mode():
         assert torch.equal(net(xs[3]), eager(xs[3]))
+
+
+@gpu
+def test_module_on_two_streams_at_once():
+    net = small_renderer(precision="int8")
+    xs = [features((2, 36, 16, 16), 1, 40 + i).to(DEV) for i in range(2)]
+    with torch.no_grad():
+        want = [net(x) for x in xs]
+        torch.cuda.synchronize()
+        streams, got = [torch.cuda.Stream() for _ in xs], [[], []]
+        for turn in range(6):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got[i].append(net(xs[(i + turn) % 2]))
+        torch.cuda.synchronize()
+    assert all(torch.equal(got[i][turn], want[(i + turn) % 2]) for i in range(2) for turn in range(6))
+    assert len(net._int8.streams) == 3
+
+
+@gpu
+@pytest.mark.parametrize("warm", [False, True])
+def test_module_captured_by_a_caller(warm):
+    """The caller's own graph quantises the weights: replays follow an in-place update, and an eager call before the first replay does not
+    take weights that were only recorded."""
+    net = small_renderer(precision="int8")
+    static, xs = features((1, 36, 16, 16), 1, 50).to(DEV), [features((1, 36, 16, 16), 1, 51 + i).to(DEV) for i in range(3)]
+    eager = lambda x: G.neural_render_int8(x, {k: v for k, v in net.named_parameters() if k != "bg_featmap"}, 2, 8)
+    with torch.no_grad():
+        want = eager(xs[0])                                                     # the library is loaded
+        if warm:
+            net(static)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = net(static)
+        assert torch.equal(net(xs[0]), want)
+        for turn in range(3):
+            for x in xs:
+                static.copy_(x)
+                graph.replay()
+                got = out.clone()
+                torch.cuda.synchronize()
+                assert torch.equal(got, eager(x)) and torch.equal(net(x), got)
+            net.feat_upsample_list[0].layer_1.weight.mul_(1.25)
+
+
+@gpu
+def test_module_made_in_inference_mode():
+    """Writes to tensors made in inference mode are not counted: the weights are quantised in every call."""
+    with torch.inference_mode():
+        net = small_renderer(precision="int8")
+        x = features((1, 36, 16, 16), 1, 60).to(DEV)
+        for _ in range(2):
+            assert torch.equal(net(x), G.neural_render_int8(x, {k: v for k, v in net.named_parameters() if k != "bg_featmap"}, 2, 8))
+            net.feat_layers[0].weight.mul_(1.5)
+
+
+def test_module_copies():
+    """Copies and pickles start without captured graphs; a module pickled before there was a precision is an fp32 one."""
+    net = small_renderer("cpu", precision="int8")
+    for twin in (copy.deepcopy(net), pickle.loads(pickle.dumps(net))):
+        assert twin.precision == "int8" and not twin._int8.streams and twin._int8 is not net._int8
+    state = dict(net.__dict__)
+    del state["precision"], state["_int8"]
+    old = G.NeuralRendererAMD.__new__(G.NeuralRendererAMD)
+    old.__setstate__(state)
+    assert old.precision == "fp32" and not old._int8.streams and old.eval() is old
 
 
 @gpu
