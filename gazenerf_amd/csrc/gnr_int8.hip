@@ -204,7 +204,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void int8_tile_kernel(const Int8Ar
 
     // epilogue: scale, bias, activation in fp32; 32 rows of n x EM values turn in LDS so that a row leaves as whole lines
     char* turn = lds + wave * 4096;
-    const bool inside = m0 + BM <= M && n0 + BN <= N, lines = M * sizeof(T) % 128 == 0;
+    // past the caches: whole lines, or a y that does not fit them anyway (53528 x 624 -> 4092, 438 MB of partial lines: 219 / 249 us)
+    const bool inside = m0 + BM <= M && n0 + BN <= N, past = M * sizeof(T) % 128 == 0 || a.N * a.O * (long)sizeof(T) >= CACHES;
     const int mw = 32 * TM * wm;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
@@ -238,7 +239,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void int8_tile_kernel(const Int8Ar
                     __builtin_memcpy(&o, __builtin_assume_aligned(turn + row * RB + 16 * (pc ^ (row & (PPR - 1))), 16), 16);
                     const int ml = 32 * (i - PAIR + 1) + Vec<T>::N * pc;
                     T* p = yn + row * M + ml;
-                    if (inside && lines) store_part<true>(p, o, Vec<T>::N);
+                    if (inside && past) store_part<true>(p, o, Vec<T>::N);
                     else if (inside) store_part(p, o, Vec<T>::N);
                     else if (n0 + nl + row < N && m0 + mw + ml < M) {
                         const long left = M - m0 - mw - ml;
@@ -632,6 +633,7 @@ static int int8_fuse(const GnrInt8Problem* p) {
     const int vec = p->x_type == GNR_F32 ? 4 : 8;
     int nmt = p->o <= 32 ? 4 : (p->o <= 64 ? 2 : 1), span;
     while (cf && nmt > 1 && p->k > 32 * vec * 4 / nmt) nmt /= 2;               // maps: 4 quads of channels a thread
+    while (nmt > 1 && N < 32 * 256 * nmt) nmt /= 2;                            // a workgroup for every CU first
     if (cf && p->k > 32 * vec * 4 / nmt) return FUSE_NONE;
     const long groups = cf ? p->batch * ((p->n_pix + 32 * nmt - 1) / (32 * nmt)) : (N + 32 * nmt - 1) / (32 * nmt), parts = fused_parts(p->o, nmt, &span);
     if (groups * parts * 256 >= (1L << 32)) return FUSE_NONE;                  // check_grid
@@ -671,8 +673,9 @@ template <typename X, typename T, bool CF, int TT> static void launch_few(const 
 // Which kernel.  Figures: us on one card, bf16 y unless stated, rows x K -> O.
 //   at most 64 rows       the few-rows kernel (1 x 2048 -> 4096: 64 x 64 tiles 10)
 //   O <= 32, 64           tiles as narrow as the layer (262144 x 64 -> 32, fp32 maps: 8.0 against 9.0 with 64 rows a wave)
-//   256 x 256 tiles       where they fill the card and K is long: 16384 x 2048 -> 4096 150 against 196 with 128 x 128, but
-//                         28672 x 516 -> 1032 47 against 41: there it is y that takes the time
+//   256 x 256 tiles       where K is long, they fill the card and few of their values fall outside: 16384 x 2048 -> 4096 150 / 221
+//                         with 128 x 128, but 28672 x 516 -> 1032 (a fifth outside) 43 / 41 and 28672 x 258 -> 516 23 / 18
+//   128 x 256 rows        for K as long otherwise: 28672 x 516 -> 1032 36 / 41; with few of them 8192 x 516 -> 1032 15.8 / 15.0
 //   128 x 128, 64 x 64    by whether the larger fill the card (4096 x 258 -> 516, fp32: 64 x 64 6.2, 128 x 128 8.3)
 template <typename T, bool CF> static int launch_int8(const Int8Args& a, long batch, hipStream_t st) {
     if (a.N <= FEW_MAX) {
@@ -687,7 +690,9 @@ template <typename T, bool CF> static int launch_int8(const Int8Args& a, long ba
     constexpr int WM = CF ? 4 : 1, WN = CF ? 1 : 4;
     if (a.O <= 32) return launch_tile<T, CF, WM, WN, 1, 1, 3>(a, batch, st);
     if (a.O <= 64) return launch_tile<T, CF, WM, WN, CF ? 1 : 2, CF ? 2 : 1, 3>(a, batch, st);
-    if (t256 >= 256 && a.K >= 1024) return launch_tile<T, CF, 2, 4, 4, 2, 4>(a, batch, st);
+    if (a.K >= 512 && t256 >= 256 && t256 * 65536 / 17 <= M * N * B / 16) return launch_tile<T, CF, 4, 2, 2, 4, 4>(a, batch, st);
+    if constexpr (!CF)
+        if (a.K >= 512 && (M + 127) / 128 * ((N + 255) / 256) >= 400) return launch_tile<T, CF, 2, 2, 2, 4, 3>(a, batch, st);
     if (t128 >= 256) return launch_tile<T, CF, 2, 2, 2, 2, 3>(a, batch, st);
     return launch_tile<T, CF, 2, 2, 1, 1, 4>(a, batch, st);
 }

@@ -189,13 +189,14 @@ template <typename T> __device__ __forceinline__ T row_value(int q, float s) {
 // (339 MB): 112 us through the caches, 51 us = 6.6 TB/s past them.  (The tile -> XCD order of quant_maps_kernel costs here: 54 us.)
 // ---------------------------------------------------------------------------------------------
 template <typename T, int LPX>
-__global__ __launch_bounds__(256) void read_maps_kernel(const GnrRowsProblem p, unsigned tiles, int ld, int step) {
+__global__ __launch_bounds__(256) void read_maps_kernel(const GnrRowsProblem p, unsigned tiles, unsigned parts, int ld, int step) {
     constexpr int V = Vec<T>::N, TP = LPX * V, U = 4;
     extern __shared__ unsigned smem[];                      // [TP][ld]
     const int NT = (int)blockDim.x, G = NT / LPX, tid = (int)threadIdx.x, l = tid % LPX, g = tid / LPX;
     // maps whose channels are whole lines: past the caches, any order.  Others: neighbouring tiles share lines, which one L2 puts together
+    // (64 maps of 258 x 4095, fp32: 93 us, past the caches 159)
     const bool lines = (p.x_stride * (long)sizeof(T)) % 128 == 0;
-    const unsigned at = lines ? blockIdx.x : xcd_block(gridDim.x);
+    const unsigned blk = lines ? blockIdx.x : xcd_block(gridDim.x), at = blk / parts;
     const long b = at / tiles, p0 = tile_start(at % tiles, TP, p.n_pix);
     const SlotRef ref = slot_of(p.slots, p.n_slots, b);
     const int C = p.channels, rows = p.n_pix - p0 < TP ? (int)(p.n_pix - p0) : TP;
@@ -208,9 +209,9 @@ __global__ __launch_bounds__(256) void read_maps_kernel(const GnrRowsProblem p, 
     for (int v = 0; v < V; ++v)
         s[v] = ref.state ? (ref.state == 1 ? 0.0f : __uint_as_float(0x7fc00000u)) : (v < nv ? p.scale[ref.slot * p.scale_batch + pl + v] : 0.0f);
     T* yb = (T*)p.x + b * p.x_batch + pl;
-    for (int c0 = 0; c0 < C; c0 += step) {                  // once, unless the rows of a tile exceed the LDS
+    for (int c0 = (int)(blk % parts) * step; c0 < C; c0 += (int)parts * step) {      // once, unless the rows of a tile exceed the LDS
         const int cols = C - c0 < step ? C - c0 : step, per_row = (cols + 15) >> 4, n = ref.state ? 0 : rows * per_row;
-        if (c0) __syncthreads();
+        if (c0 >= (int)parts * step) __syncthreads();
         for (int i0 = tid; i0 < n; i0 += NT * U) {
             Vec<int8_t> o[U];
 #pragma unroll
@@ -281,7 +282,8 @@ template <typename T, int LPX> static int quant_maps_lpx(const GnrRowsProblem& p
 #undef GNR_MAPS
     return 0;
 }
-// 32 pixels a tile, 16 where an fp32 map would leave half the CUs without one (one map of 258 x 4096: 5.1 / 5.5 us).  Threads: the fewest that
+// 32 pixels a tile, 16 where they would leave CUs without one (one map of 258 x 4096 in fp32: 5.1 / 5.5 us, two of 690 x 900 in bf16: 6.6 / 7.5;
+// five of 129 x 1369 in bf16 the other way round: 6.3 / 5.9).  Threads: the fewest that
 // keep a row in 4 quads of channels each (64 such maps: 78 us with 256 threads, 84 with 512), twice that while there are few of them (one
 // map: 6.8 / 5.5; five of 129 x 1369, bf16: 6.9 / 5.9).
 template <typename T> static int quant_maps(const GnrRowsProblem& p, hipStream_t st) {
@@ -291,7 +293,7 @@ template <typename T> static int quant_maps(const GnrRowsProblem& p, hipStream_t
     int nt = 64;
     while (nt < 1024 && quads > nt / LPX * 4) nt *= 2;
     while (nt < 512 && tiles * nt < 131072 && quads > nt / LPX) nt *= 2;
-    if (sizeof(T) == 4 && tiles < 192 && nt > 64) return quant_maps_lpx<T, 4>(p, nt, st);
+    if (tiles < (sizeof(T) == 4 ? 192 : 128) && nt > 64) return quant_maps_lpx<T, LPX / 2>(p, nt, st);
     return quant_maps_lpx<T, LPX>(p, nt, st);
 }
 
@@ -331,20 +333,24 @@ int launch_quantize(const GnrRowsProblem& p, hipStream_t st) {
     return e == hipSuccess ? 0 : fail("gnr_quantize_rows: launch failed: %s", hipGetErrorString(e));
 }
 
-template <typename T, int LPX> static int read_maps_lpx(const GnrRowsProblem& p, hipStream_t st) {
+template <typename T, int LPX> static int read_maps_lpx(const GnrRowsProblem& p, int want, hipStream_t st) {
     constexpr int TP = LPX * Vec<T>::N;
     const unsigned tiles = (unsigned)((p.n_pix + TP - 1) / TP);
-    const int step = p.channels < 1920 ? p.channels : 1920, ld = (step + 63) / 64 * 16 + 4;
+    int step = ((p.channels + want - 1) / want + 63) / 64 * 64;
+    step = step < 1920 ? step : 1920;
+    const unsigned parts = (unsigned)(want > 1 ? (p.channels + step - 1) / step : 1);
+    const int ld = step / 4 + 4;
     int nt = 64;                                               // a quad of channels a thread and turn: no more threads than quads
-    while (nt < 256 && (p.channels + 3) / 4 > nt / LPX) nt *= 2;
-    if (check_grid("gnr_read_rows", (long)tiles * p.batch, nt)) return 1;
-    hipLaunchKernelGGL((read_maps_kernel<T, LPX>), dim3(tiles * (unsigned)p.batch), dim3((unsigned)nt), sizeof(unsigned) * TP * ld, st, p, tiles, ld, step);
+    while (nt < 256 && (step < p.channels ? step : p.channels) > nt / LPX * 4) nt *= 2;
+    if (check_grid("gnr_read_rows", (long)tiles * p.batch * parts, nt)) return 1;
+    hipLaunchKernelGGL((read_maps_kernel<T, LPX>), dim3(tiles * (unsigned)p.batch * parts), dim3((unsigned)nt), sizeof(unsigned) * TP * ld, st, p,
+                       tiles, parts, ld, step);
     return 0;
 }
-// 32 pixels a tile; 16 in fp32 while there are few (two maps of 258 x 4096: 5.5 / 6.6 us, 64: 52.7 / 51.4)
+// 32 pixels a tile; while there are few, up to eight workgroups share one's channels (258 x 4096 in fp32, one map: 3.6 / 6.1 us, four: 4.7 / 6.2,
+// sixteen: 17.1 / 15.2; two of 690 x 900 in bf16: 4.2 / 9.9)
 template <typename T> static int read_maps(const GnrRowsProblem& p, hipStream_t st) {
-    if (sizeof(T) == 2 || (p.n_pix + 31) / 32 * p.batch < 2048) return read_maps_lpx<T, 4>(p, st);
-    return read_maps_lpx<T, 8>(p, st);
+    return read_maps_lpx<T, 32 / (sizeof(T) == 4 ? 4 : 8)>(p, (p.n_pix + 31) / 32 * p.batch < 1024 ? 8 : 1, st);
 }
 
 }  // namespace gnr
