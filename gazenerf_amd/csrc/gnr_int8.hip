@@ -614,8 +614,9 @@ static int check_int8(const GnrInt8Problem* p) {
 // Which kernel takes floating x as it is (FUSE_NONE: x is quantised into the workspace first), us by fused / two launches:
 //   FUSE_FEW  rows that the few-rows kernel takes
 //   1 2 4     int8_fused_kernel with that many 32-row tiles a workgroup
-// Up to 128 outputs a workgroup multiplies with all of them: 1 + 1 / 128 .. reads of x, no 8-bit rows in memory (262144 x 64 -> 32, fp32
-// maps: 18.8 / 27.9), with as many row tiles as keep four waves busy, fewer where a row of K does not fit a thread's registers.
+// Up to 128 outputs a workgroup multiplies with all of them: x is read once and its 8-bit rows never reach memory (262144 x 64 -> 32, fp32
+// maps: 18.8 / 27.9), with as many row tiles as keep four waves busy, fewer where a row of K does not fit a thread's registers or CUs would
+// be left without a workgroup (1028 x 396 -> 16, fp32: one tile 5.8, four 11.2).
 // Beyond, every workgroup takes four output tiles and the rows are quantised again for each: only while there is a CU for every workgroup,
 // when what counts is one launch instead of two (88 x 456 -> 1701, fp16: 6.7 / 10.4; 4096 x 258 -> 516, 640 workgroups: 11.5 / 10.1).
 enum { FUSE_NONE = 0, FUSE_FEW = 8 };
@@ -671,7 +672,7 @@ template <typename X, typename T, bool CF, int TT> static void launch_few(const 
 }
 
 // Which kernel.  Figures: us on one card, bf16 y unless stated, rows x K -> O.
-//   at most 64 rows       the few-rows kernel (1 x 2048 -> 4096: 64 x 64 tiles 10)
+//   at most 64 rows       the few-rows kernel (1 x 2048 -> 4096: 4.4 / 10 with 64 x 64 tiles)
 //   O <= 32, 64           tiles as narrow as the layer (262144 x 64 -> 32, fp32 maps: 8.0 against 9.0 with 64 rows a wave)
 //   256 x 256 tiles       where K is long, they fill the card and few of their values fall outside: 16384 x 2048 -> 4096 150 / 221
 //                         with 128 x 128, but 28672 x 516 -> 1032 (a fifth outside) 43 / 41 and 28672 x 258 -> 516 23 / 18
