@@ -204,8 +204,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void int8_tile_kernel(const Int8Ar
 
     // epilogue: scale, bias, activation in fp32; 32 rows of n x EM values turn in LDS so that a row leaves as whole lines
     char* turn = lds + wave * 4096;
-    // past the caches: whole lines, or a y that does not fit them anyway (53528 x 624 -> 4092, 438 MB of partial lines: 219 / 249 us)
-    const bool inside = m0 + BM <= M && n0 + BN <= N, past = M * sizeof(T) % 128 == 0 || a.N * a.O * (long)sizeof(T) >= CACHES;
+    // past the caches: whole lines, or 16-bit rows that do not fit them anyway (53528 x 624 -> 4092, 438 MB of partial lines: 224 / 261 us; in
+    // fp32 26764 x 624 -> 4092 232 / 184, maps of 233 x 220001 -> 570 362 / 195)
+    const bool inside = m0 + BM <= M && n0 + BN <= N, past = M * sizeof(T) % 128 == 0 || (!CF && sizeof(T) == 2 && a.N * a.O * (long)sizeof(T) >= CACHES);
     const int mw = 32 * TM * wm;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void int8_tile_kernel(const Int8Ar
 }
 
 // ---------------------------------------------------------------------------------------------
-// few rows (at most 16 TT): the time to read the weights.  A workgroup owns 16 outputs; its four waves share K in steps of 64 bytes
+// few rows: the time to read the weights.  A workgroup owns 16 outputs of 16 TT rows; its four waves share K in steps of 64 bytes
 // (v_mfma_i32_16x16x64_i8: lane l holds row l % 16, bytes 16 (l / 16) ..) and keep eight steps of weights in flight, fragments
 // straight from memory; the four partial sums are whole numbers and meet in LDS.  Floating x is quantised by every workgroup
 // for itself (TT == 1): one launch instead of two.
@@ -314,7 +315,8 @@ __global__ __launch_bounds__(256) void int8_few_kernel(const Int8Args a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];                 // FLOAT: rows of x, [16][ld]; then the partial sums
     __shared__ float xsc[16 * TT];
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, kq = 16 * (lane >> 4);
-    const int N = (int)a.N, K = a.K, K16 = (K + 15) & ~15, nst = (K + 63) / 64, o0 = (int)blockIdx.x * 16;
+    const long n0 = (long)blockIdx.y * 16 * TT;                // FLOAT: 0
+    const int N = a.N - n0 < 16 * TT ? (int)(a.N - n0) : 16 * TT, K = a.K, K16 = (K + 15) & ~15, nst = (K + 63) / 64, o0 = (int)blockIdx.x * 16;
     const int ld = nst * 64 + 16;
     const int o = o0 + col < a.O ? o0 + col : a.O - 1;
     const int8_t* wp = a.w + (long)o * a.w_pitch;
@@ -323,9 +325,9 @@ __global__ __launch_bounds__(256) void int8_few_kernel(const Int8Args a) {
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
             const int n = 16 * t + col < N ? 16 * t + col : N - 1;
-            xp[t] = x_row(a, 0, n, false);
+            xp[t] = x_row(a, 0, n0 + n, false);
         }
-        if (tid < 16 * TT) xsc[tid] = x_scale(a, 0, tid < N ? tid : N - 1, false);
+        if (tid < 16 * TT) xsc[tid] = x_scale(a, 0, n0 + (tid < N ? tid : N - 1), false);
     }
     i32x4 w[U], x[U][TT];
     auto load = [&](int s0) {
@@ -379,8 +381,8 @@ __global__ __launch_bounds__(256) void int8_few_kernel(const Int8Args a) {
         const int n = 16 * t + col;
         if (n >= N) continue;
         const float sx = xsc[n];
-        const int P = (int)a.P;
-        T* y = CF ? (T*)a.y + (long)(n / P) * a.O * P + n % P : (T*)a.y + (long)n * a.O;
+        const unsigned P = (unsigned)a.P, at = (unsigned)(n0 + n);
+        T* y = CF ? (T*)a.y + (long)(at / P) * a.O * P + at % P : (T*)a.y + (n0 + n) * a.O;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int oo = o0 + 4 * (lane >> 4) + r;
@@ -667,21 +669,24 @@ template <typename T, bool CF, int WM, int WN, int TM, int TN, int NST = 4> stat
 
 template <typename X, typename T, bool CF, int TT> static void launch_few(const Int8Args& a, hipStream_t st) {
     const int rows = 16 * (((a.K + 63) / 64) * 64 + 16), part = 4 * TT * 64 * 16;
-    hipLaunchKernelGGL((int8_few_kernel<X, T, CF, TT>), dim3((unsigned)((a.O + 15) / 16)), dim3(256),
+    hipLaunchKernelGGL((int8_few_kernel<X, T, CF, TT>), dim3((unsigned)((a.O + 15) / 16), (unsigned)((a.N + 16 * TT - 1) / (16 * TT))), dim3(256),
                        !__is_same(X, int8_t) && rows > part ? rows : part, st, a);
 }
 
 // Which kernel.  Figures: us on one card, bf16 y unless stated, rows x K -> O.
 //   at most 64 rows       the few-rows kernel (1 x 2048 -> 4096: 4.4 / 10 with 64 x 64 tiles)
+//   little of y           the same with blocks of 16 or 32 rows, while a CU has about one: what counts is how K is shared (150 x 1422 -> 256: 4.0 /
+//                         6.5, 100 x 2048 -> 834: 6.3 / 8.0; 512 x 2048 -> 834, 848 blocks of 32: 14.8 / 8.2)
 //   O <= 32, 64           tiles as narrow as the layer (262144 x 64 -> 32, fp32 maps: 8.0 against 9.0 with 64 rows a wave)
 //   256 x 256 tiles       where K is long, they fill the card and few of their values fall outside: 16384 x 2048 -> 4096 150 / 221
 //                         with 128 x 128, but 28672 x 516 -> 1032 (a fifth outside) 43 / 41 and 28672 x 258 -> 516 23 / 18
 //   128 x 256 rows        for K as long otherwise: 28672 x 516 -> 1032 36 / 41; with few of them 8192 x 516 -> 1032 15.8 / 15.0
 //   128 x 128, 64 x 64    by whether the larger fill the card (4096 x 258 -> 516, fp32: 64 x 64 6.2, 128 x 128 8.3)
 template <typename T, bool CF> static int launch_int8(const Int8Args& a, long batch, hipStream_t st) {
-    if (a.N <= FEW_MAX) {
-        if (a.N <= 16) launch_few<int8_t, T, CF, 1>(a, st);
-        else if (a.N <= 32) launch_few<int8_t, T, CF, 2>(a, st);
+    const long few = (a.N + 15) / 16 * ((a.O + 15) / 16), few2 = (a.N + 31) / 32 * ((a.O + 15) / 16);
+    if (a.N <= FEW_MAX || few2 <= 320) {
+        if (a.N <= 16 || few <= 256) launch_few<int8_t, T, CF, 1>(a, st);
+        else if (a.N <= 32 || few2 <= 320) launch_few<int8_t, T, CF, 2>(a, st);
         else launch_few<int8_t, T, CF, 4>(a, st);
         return 0;
     }

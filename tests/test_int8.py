@@ -481,6 +481,28 @@ def test_linear_maps(b, k, o, p, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("n, k, o", [
+    (150, 1430, 250), (100, 2050, 834), (30, 100, 9000), (64, 40, 5000),         # blocks of 16, 32 and 64 rows whose waves share K
+    (1030, 129, 259), (9000, 48, 31), (5000, 130, 63),                           # 64 x 64 tiles, layers of at most 32 and 64 outputs
+    (4100, 70, 1030), (6500, 517, 2050), (4090, 515, 4090)])                     # 128 x 128, 128 x 256, 256 x 256 tiles
+def test_linear_every_tile(n, k, o):
+    """8-bit rows with bytes behind their channels, as rows and as two maps, every type of result; the sums in 64 bits (whole numbers: exact)."""
+    g = gen(n + k + o)
+    x = torch.randint(-128, 128, (n, int8.row_pitch(k, 16)), generator=g, dtype=torch.int8).to(DEV)[:, :k]
+    w = torch.randint(-128, 128, (o, int8.row_pitch(k, 16)), generator=g, dtype=torch.int8).to(DEV)[:, :k]
+    xs, ws, b = torch.rand(n, generator=g) * 0.02, torch.rand(o, generator=g) * 0.02, torch.randn(o, generator=g)
+    xs[n // 2], xs[n - 1] = 0.0, math.nan
+    t = (x.double() @ w.double().t()).cpu() * xs.double()[:, None] * ws.double()
+    y = t + b.double()
+    ref, bound = torch.where(y < 0, y * 0.2, y), 6 * 2.0 ** -24 * (t.abs() + b.double().abs())
+    args = w, ws.to(DEV), b.to(DEV)
+    for out in (torch.float32, torch.bfloat16, torch.float16):
+        assert_linear(G.int8_linear(x, *args, x_scale=xs.to(DEV), leaky=True, out_dtype=out), ref, bound)
+        maps = G.int8_linear(x.view(2, n // 2, k), *args, x_scale=xs.to(DEV).view(2, -1), leaky=True, channels_first=True, out_dtype=out)
+        assert_linear(maps.transpose(1, 2).reshape(n, o), ref, bound)
+
+
+@gpu
 def test_linear_any_bytes():
     """8-bit rows a caller made (the value -128, bytes behind the channels that are not zero), sums that need more than 24 bits."""
     for n, k, o in ((5, 130000, 3), (300, 2050, 70), (1, 999, 40)):
