@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import threading
 from typing import Dict
 
 import torch
@@ -145,6 +146,20 @@ def neural_render(x, params: Dict[str, torch.Tensor], n_blocks: int = 3, min_fea
     names = renderer_param_names(n_blocks)
     cfg = dict(n_blocks=int(n_blocks), min_feat=int(min_feat), final_actvn=bool(final_actvn))
     return _UpsampleFn.apply(cfg, x, *[params[n] for n in names])
+
+
+# Captures of this package run one at a time: torch.cuda.graph captures on ONE side stream that all threads share.  Other threads may go on
+# allocating and launching meanwhile (capture_error_mode="thread_local"; torch's own default forbids it to the whole process).
+_CAPTURE = threading.Lock()
+
+
+def capture_graph(call):
+    """``call()`` recorded into a new ``torch.cuda.CUDAGraph`` on the current device."""
+    with _CAPTURE:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+            call()
+    return graph
 
 
 class GraphedUpsample:

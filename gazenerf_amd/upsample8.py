@@ -8,13 +8,14 @@ reads as they are; both give the same image bit for bit.  There is no backward.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from typing import Dict, Optional
 
 import torch
 
 from . import _lib, int8
 from .render import _check_tensor, _stream_ptr
-from .upsample import _expected_shapes, _weights_struct, renderer_param_names
+from .upsample import _expected_shapes, _weights_struct, capture_graph, renderer_param_names
 
 _CONVS = (("up1", "feat_upsample_list.%d.layer_1"), ("up2", "feat_upsample_list.%d.layer_2"), ("feat", "feat_layers.%d"))
 
@@ -23,15 +24,20 @@ class Int8Weights:
     """The renderer's convolution weights as 8-bit rows, quantised once and again when a parameter changed: another tensor, a
     higher ``_version`` (torch counts every in-place write) or another ``data_ptr()``.  An in-place write through ``.data`` is invisible to
     all three, and so is one by a replayed graph: call ``clear()`` after one.  The buffers stay where they are while shapes and device do,
-    so captured graphs that read them see the new values.  One per module and HIP stream (``Int8Renderers``)."""
+    so captured graphs that read them see the new values.  One per module and HIP stream (``Int8Renderers``); threads that share it
+    hold ``lock`` from ``refresh`` until they have what they took from it."""
 
     def __init__(self):
+        self.lock = threading.RLock()
+        self.clear()
+
+    def clear(self):
         self.rows: Dict[str, int8.QuantizedRows] = {}
         self.seen = None
         self.quantised = 0
 
-    def clear(self):
-        self.__init__()
+    def __reduce__(self):                          # a copy or a pickle starts empty, with a lock of its own
+        return Int8Weights, ()
 
     def refresh(self, params: Dict[str, torch.Tensor], n_blocks: int) -> None:
         names = [name % i for i in range(n_blocks) for _, name in _CONVS]
@@ -100,11 +106,13 @@ class _Call:
         if B < 1:
             raise ValueError("empty batch")
         self.params = _checked_params(params, Cn, n_blocks, min_feat, dev)
-        weights.refresh(params, n_blocks)
         self.p, self.s = _lib.GnrUpsampleProblem(), _lib.GnrUpsampleInt8()
         p, s = self.p, self.s
+        with weights.lock:
+            weights.refresh(params, n_blocks)
+            weights.fill(s, n_blocks)
+            self.rows = dict(weights.rows)
         p.batch, p.feat_nc, p.featmap_size, p.n_blocks, p.min_feat, p.final_sigmoid = B, Cn, S, n_blocks, min_feat, int(final_actvn)
-        weights.fill(s, n_blocks)
         if x is not None:
             self.x = x.detach().contiguous()
             p.x = self.x.data_ptr()
@@ -115,7 +123,6 @@ class _Call:
             s.x_q, s.x_batch, s.x_pitch = q.data_ptr(), int8._stride(q, 0, 0), int8._stride(q, 1, int8.row_pitch(Cn))
             s.x_scale, s.x_scale_batch, s.slots, s.n_slots = scale.data_ptr(), int(scale.stride(0)), self.x.data_ptr(), q.shape[0]
         self.w = _weights_struct(self.params, n_blocks)
-        self.rows = dict(weights.rows)
         self.dev = dev
         lib = _lib.load()
         need = lib.gnr_upsample_int8_workspace_bytes(C.byref(p), C.byref(s))
@@ -147,10 +154,13 @@ def neural_render_int8(x, params: Dict[str, torch.Tensor], n_blocks: int = 3, mi
 class GraphedUpsample8:
     """``neural_render_int8`` replayed from a HIP graph, one per input shape (or cache), device and parameter storage: the call is
     some thirty launches of a few microseconds.  The graph reads the quantised weights of ``weights``, refreshed before each replay if a
-    parameter changed, and the biases and RGB weights in place; the input (a map, or the slots) is copied into the graph's own buffer."""
+    parameter changed, and the biases and RGB weights in place; the input (a map, or the slots) is copied into the graph's own buffer.
+    For one HIP stream, from any number of threads: between a call's copy into that buffer and its copy out of the image nobody else's
+    work is enqueued."""
 
     def __init__(self, weights: Int8Weights, max_entries: int = 4):
         self.weights, self.max_entries = weights, max_entries
+        self.lock = threading.Lock()
         self.entries = {}
         self.captures = self.replays = 0
 
@@ -158,6 +168,10 @@ class GraphedUpsample8:
         self.entries.clear()
 
     def __call__(self, params, n_blocks, min_feat, final_actvn, x=None, cache=None, slots=None):
+        with self.lock, self.weights.lock:
+            return self._replay(params, n_blocks, min_feat, final_actvn, x, cache, slots)
+
+    def _replay(self, params, n_blocks, min_feat, final_actvn, x, cache, slots):
         self.weights.refresh(params, n_blocks)
         given = x if x is not None else slots
         key = (tuple(given.shape), given.dtype, given.device, n_blocks, min_feat, bool(final_actvn)) + tuple(
@@ -194,9 +208,7 @@ class GraphedUpsample8:
             with torch.cuda.stream(side):
                 call()                                               # warm-up outside the capture
             torch.cuda.current_stream(dev).wait_stream(side)
-            graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph):
-                call()
+            graph = capture_graph(call)
         self.captures += 1
         return graph, static, call
 
@@ -208,24 +220,29 @@ class Int8Renderers:
     def __init__(self, max_streams: int = 4):
         self.max_streams = max_streams
         self.streams = {}
+        self.lock = threading.Lock()
 
     def __call__(self, dev) -> GraphedUpsample8:
         key = torch.cuda.current_stream(dev).cuda_stream if dev.type == "cuda" else None
-        r = self.streams.pop((dev, key), None)
-        if r is None:
-            r = GraphedUpsample8(Int8Weights())
-            while len(self.streams) >= self.max_streams:
-                self.streams.pop(next(iter(self.streams)))
-        self.streams[dev, key] = r
+        with self.lock:
+            r = self.streams.pop((dev, key), None)
+            if r is None:
+                r = GraphedUpsample8(Int8Weights())
+                while len(self.streams) >= self.max_streams:
+                    self.streams.pop(next(iter(self.streams)))
+            self.streams[dev, key] = r
         return r
 
     def look_again(self):
         """The next call on each stream quantises its weights again."""
-        for r in self.streams.values():
-            r.weights.seen = None
+        with self.lock:
+            for r in self.streams.values():
+                with r.weights.lock:
+                    r.weights.seen = None
 
     def clear(self):
-        self.streams.clear()
+        with self.lock:
+            self.streams.clear()
 
     def __deepcopy__(self, memo):
         return Int8Renderers(self.max_streams)

@@ -8,13 +8,15 @@ the sigmoid (slope at most 1/4, expf and the quotient within 4 u of a value belo
 import copy
 import ctypes as C
 import pickle
+import sys
+import threading
 
 import pytest
 import torch
 import torch.nn.functional as F
 
 import gazenerf_amd as G
-from gazenerf_amd import _lib
+from gazenerf_amd import _lib, upsample8
 from gazenerf_amd.upsample import _channels, _expected_shapes, renderer_param_names
 from test_int8 import DEV, features, gen, ref_rows
 
@@ -188,6 +190,87 @@ def test_module_on_two_streams_at_once():
         torch.cuda.synchronize()
     assert all(torch.equal(got[i][turn], want[(i + turn) % 2]) for i in range(2) for turn in range(6))
     assert len(net._int8.streams) == 3
+
+
+def in_threads(n, work):
+    """work(i) in n threads at once, with the interpreter switching between them as often as it can; their results in order."""
+    out, errors, start = [None] * n, [], threading.Barrier(n)
+
+    def body(i):
+        try:
+            start.wait()
+            out[i] = work(i)
+        except BaseException as e:
+            errors.append(e)
+    every = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    try:
+        threads = [threading.Thread(target=body, args=(i,)) for i in range(n)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    finally:
+        sys.setswitchinterval(every)
+    if errors:
+        raise errors[0]
+    return out
+
+
+def test_replays_of_two_threads_stay_apart():
+    """The replay's own steps -- copy in, replay, copy out -- with a stand-in for the graph and its tensors on the CPU: each thread gets what
+    belongs to its input."""
+    class Replay:
+        def __init__(self, static, img):
+            self.static, self.img = static, img
+
+        def replay(self):
+            self.img.copy_(self.static * 2)
+
+    class OnCpu(upsample8.GraphedUpsample8):
+        def _capture(self, params, n_blocks, min_feat, final_actvn, x, cache, slots):
+            static, call = torch.empty_like(x), type("Call", (), {"img": torch.empty_like(x)})()
+            self.captures += 1
+            return Replay(static, call.img), static, call
+
+    class NoWeights(upsample8.Int8Weights):
+        def refresh(self, params, n_blocks):
+            pass
+
+    graphed = OnCpu(NoWeights())
+    params = {n: torch.zeros(1) for n in renderer_param_names(1)}
+
+    def work(i):
+        x = torch.full((4,), float(i + 1))
+        return sum(not torch.equal(graphed(params, 1, 8, True, x=x), 2 * x) for _ in range(3000))
+    assert in_threads(2, work) == [0, 0] and graphed.captures == 1
+
+
+def test_weights_copy_empty():
+    """Int8Weights and its lock: copies and pickles start empty."""
+    w = upsample8.Int8Weights()
+    w.quantised, w.rows["x"] = 3, None
+    for twin in (copy.deepcopy(w), pickle.loads(pickle.dumps(w))):
+        assert not twin.rows and twin.seen is None and twin.quantised == 0 and twin.lock is not w.lock
+
+
+@gpu
+@pytest.mark.parametrize("own_streams", [False, True])
+def test_module_in_threads(own_streams):
+    """Three threads, each with its own map, on the default stream and on streams of their own; the graphs are captured while the others run."""
+    net = small_renderer(precision="int8")
+    xs = [features((1 + (i == 2), 36, 16, 16), 1, 70 + i).to(DEV) for i in range(3)]
+    params = {k: v for k, v in net.named_parameters() if k != "bg_featmap"}
+    with torch.no_grad():
+        want = [G.neural_render_int8(x, params, 2, 8) for x in xs]
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.no_grad(), torch.cuda.stream(torch.cuda.Stream() if own_streams else torch.cuda.current_stream()):
+            got = [net(xs[i]) for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+        return all(torch.equal(g, want[i]) for g in got)
+    assert in_threads(3, work) == [True] * 3
 
 
 @gpu
