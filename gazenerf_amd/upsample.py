@@ -168,14 +168,17 @@ class GraphedUpsample:
     One ``gnr_upsample_fwd`` call is 20 kernel launches; at B = 1 (the reference's render loops,
     utils/render_utils.py:199-219) 110 of its 512 us were the gaps between them.  The library makes no host
     synchronisation and takes every buffer from the caller, so the call captures as is: static input, workspace and image
-    buffers, one ``torch.cuda.CUDAGraph`` per (input shape, device, parameter storage).  The weight re-layout
+    buffers, one ``torch.cuda.CUDAGraph`` per (input shape, device, HIP stream, parameter storage): what two streams run at
+    once shares no buffer, and threads on one stream take turns from the copy into the static input to the copy out of the
+    static image.  The weight re-layout
     (``conv16_pack_kernel``) is INSIDE the graph, so in-place parameter updates are seen by the next replay; a parameter
     that moves to other storage (``.to()``, ``load_state_dict`` into new tensors, ``p.data = ...``) changes the key and the
     forward is captured again.  Inference only: nothing is saved for a backward."""
 
-    def __init__(self, max_entries: int = 4):
+    def __init__(self, max_entries: int = 8):
         self.entries = {}
         self.max_entries = max_entries
+        self.lock = threading.Lock()
         self.captures = 0
         self.replays = 0
 
@@ -191,24 +194,26 @@ class GraphedUpsample:
         return {"max_entries": self.max_entries}
 
     def __setstate__(self, state):
-        self.__init__(state.get("max_entries", 4))
+        self.__init__(state.get("max_entries", 8))
 
     def __call__(self, x, params: Dict[str, torch.Tensor], n_blocks: int, min_feat: int, final_actvn: bool, copy_output: bool = True):
         names = renderer_param_names(n_blocks)
         flat = [params[n] for n in names]
-        key = (tuple(x.shape), x.device, n_blocks, min_feat, bool(final_actvn)) + tuple(t.data_ptr() for t in flat) + \
+        stream = torch.cuda.current_stream(x.device).cuda_stream if x.is_cuda else None
+        key = (tuple(x.shape), x.device, stream, n_blocks, min_feat, bool(final_actvn)) + tuple(t.data_ptr() for t in flat) + \
             tuple(tuple(t.shape) for t in flat)
-        ent = self.entries.get(key)
-        if ent is None:
-            ent = self._capture(x, flat, dict(n_blocks=int(n_blocks), min_feat=int(min_feat), final_actvn=bool(final_actvn)))
-            if len(self.entries) >= self.max_entries:
-                self.entries.pop(next(iter(self.entries)))
-            self.entries[key] = ent
-        graph, x_static, img_static = ent[:3]
-        x_static.copy_(x)
-        graph.replay()
-        self.replays += 1
-        return img_static.clone() if copy_output else img_static
+        with self.lock:
+            ent = self.entries.get(key)
+            if ent is None:
+                ent = self._capture(x, flat, dict(n_blocks=int(n_blocks), min_feat=int(min_feat), final_actvn=bool(final_actvn)))
+                if len(self.entries) >= self.max_entries:
+                    self.entries.pop(next(iter(self.entries)))
+                self.entries[key] = ent
+            graph, x_static, img_static = ent[:3]
+            x_static.copy_(x)
+            graph.replay()
+            self.replays += 1
+            return img_static.clone() if copy_output else img_static
 
     def _capture(self, x, flat, cfg):
         lib = _lib.load()
@@ -242,9 +247,7 @@ class GraphedUpsample:
             with torch.cuda.stream(side):
                 call()                                  # warm-up outside the capture (module load, argument errors)
             torch.cuda.current_stream(dev).wait_stream(side)
-            graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph):
-                call()
+            graph = capture_graph(call)
         self.captures += 1
         return graph, x_static, img, ws, params, p, w      # the graph's kernels point into all of these: keep them alive
 

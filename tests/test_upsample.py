@@ -398,3 +398,86 @@ def test_graph_cache_under_inference_mode_then_no_grad_and_module_copies():
     again = torch.load(buf, weights_only=False)
     with torch.no_grad():
         assert torch.equal(again(x), b)
+
+
+def _two_threads(work):
+    import sys
+    import threading
+    out, errors, start = [None, None], [], threading.Barrier(2)
+
+    def body(i):
+        try:
+            start.wait()
+            out[i] = work(i)
+        except BaseException as e:
+            errors.append(e)
+    every = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)                      # the interpreter switches threads as often as it can
+    try:
+        threads = [threading.Thread(target=body, args=(i,)) for i in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    finally:
+        sys.setswitchinterval(every)
+    if errors:
+        raise errors[0]
+    return out
+
+
+def test_graph_replays_of_two_threads_stay_apart():
+    """GraphedUpsample's own steps -- copy in, replay, copy out -- with a stand-in for the graph on the CPU: each thread gets the
+    image of its own input."""
+    from gazenerf_amd.upsample import GraphedUpsample, renderer_param_names
+
+    class Replay:
+        def __init__(self, x, img):
+            self.x, self.img = x, img
+
+        def replay(self):
+            self.img.copy_(self.x * 2)
+
+    class OnCpu(GraphedUpsample):
+        def _capture(self, x, flat, cfg):
+            static, img = torch.empty_like(x), torch.empty_like(x)
+            self.captures += 1
+            return Replay(static, img), static, img
+
+    graphed = OnCpu()
+    params = {n: torch.zeros(1) for n in renderer_param_names(1)}
+
+    def work(i):
+        x = torch.full((4,), float(i + 1))
+        return sum(not torch.equal(graphed(x, params, 1, 8, True), 2 * x) for _ in range(3000))
+    assert _two_threads(work) == [0, 0] and graphed.captures == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("threads", [False, True])
+def test_graph_replays_on_two_streams_share_no_buffer(threads):
+    """Two streams, from one thread and from two: a graph of its own for each, every image the eager one."""
+    from gazenerf_amd import NeuralRendererAMD
+    dev = _dev()
+    torch.manual_seed(0)
+    net = NeuralRendererAMD(feat_nc=64, featmap_size=32, img_size=128, min_feat=16).to(dev).eval()
+    xs = [synth.synth_featmap(2, 64, 32, seed=s).to(dev) for s in (1, 2)]
+    want = [neural_render_eager(net, x).detach() for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    if threads:
+        def work(i):
+            with torch.no_grad(), torch.cuda.stream(streams[i]):
+                got = [net(xs[i]) for _ in range(20)]
+                streams[i].synchronize()
+            return all(torch.equal(g, want[i]) for g in got)
+        assert _two_threads(work) == [True, True]
+    else:
+        got = []
+        for turn in range(10):
+            for i, s in enumerate(streams):
+                with torch.no_grad(), torch.cuda.stream(s):
+                    got.append((net(xs[i]), want[i]))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in got)
+    assert net._graphed.captures == 2
