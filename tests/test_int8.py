@@ -571,6 +571,37 @@ def test_linear_special_values():
 
 
 @gpu
+@pytest.mark.parametrize("k", [100, 700])
+def test_linear_scales_at_the_ends_of_the_range(k):
+    """Results in range whose sum * x_scale is not: rows up to fp32's largest value times small weights, and 8-bit rows with scales of any
+    size.  The epilogue moves a power of two between the scales; every kernel, both layouts."""
+    tiny = torch.tensor([2.0 ** -149, 2.0 ** -127, 3.1e-39, 2.0 ** -107, 1.0, 2.0 ** 90, 2.0 ** 97, 1.7e38], dtype=torch.float32)
+    for n, o in ((4, 24), (40, 150), (300, 40), (700, 260), (1100, 700)):
+        x = torch.randn(n, k, generator=gen(n)).clamp(-3.3, 3.3)
+        x = x * torch.tensor([1e38, 1e37, 1e30, 1.0])[torch.arange(n) % 4].unsqueeze(1)
+        w, b = weights(o, k, 3)
+        w = w * torch.tensor([2.0 ** -12, 2.0 ** -100, 2.0 ** -40])[torch.arange(o) % 3].unsqueeze(1)
+        wq = G.quantize_rows(w.to(DEV))
+        ref, bound = linear_ref_of(x, wq.q, wq.scale, b, True)
+        assert bool((ref.abs() < 1e38).all()) and bool(((ref_rows(x)[0] @ wq.q.cpu().double().t()).abs() * ref_rows(x)[1].double()[:, None] > 1e39).any())
+        y = G.int8_linear(x.to(DEV), wq.q, wq.scale, b.to(DEV), leaky=True)
+        assert_linear(y, ref, bound)
+        y = G.int8_linear(x.t().contiguous()[None].to(DEV), wq.q, wq.scale, b.to(DEV), leaky=True, channels_first=True)
+        assert_linear(y[0].t(), ref, bound)
+
+        q, s = ref_rows(torch.randn(n, k, generator=gen(n + 1)))
+        s = tiny[torch.arange(n) % len(tiny)]
+        ws = tiny.flip(0)[torch.arange(o) % len(tiny)]
+        xq = q.to(torch.int8).to(DEV)
+        for bias in (None, b):
+            ref, bound = ref_linear(q, s, wq.q, ws, bias, False)
+            y = G.int8_linear(xq, wq.q, ws.to(DEV), None if bias is None else bias.to(DEV), x_scale=s.to(DEV))
+            assert_linear(y, ref, bound)
+            y = G.int8_linear(xq[None], wq.q, ws.to(DEV), None if bias is None else bias.to(DEV), x_scale=s[None].to(DEV), channels_first=True)
+            assert_linear(y[0].t(), ref, bound)
+
+
+@gpu
 def test_linear_output_beyond_32_bits():
     """More than 2^32 bytes of y: the rows at its end."""
     n, k, o = 1 << 20, 16, 2112
