@@ -16,7 +16,8 @@ precision="int8")`` runs its 1x1 convolutions that way.
     int8_linear(x, w_q, w_scale, bias, ...)          rows, maps or cached rows -> act(x w^T + bias)
 
 Floating tensors are float32, bfloat16 or float16.  CUDA (ROCm) tensors only; the work goes to the current stream of their
-device.  There is no backward: a call on inputs that would need a gradient is refused.
+device.  There is no backward: a call on inputs that would need a gradient, of either mode, is refused, and so is a call under
+``torch.jit.trace``, which would record its result as a constant.
 """
 from __future__ import annotations
 
@@ -27,7 +28,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib, _torch_ext
-from .render import _ext_call, _stream_ptr
+from .render import _ext_call, _has_tangent, _stream_ptr
 
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.int8: 3}
 ROW_ALIGN = 16           # rows that a product reads stand on multiples of 16 bytes (a cache: 275 bytes of 258 channels and a scale on 272 + 4)
@@ -70,6 +71,10 @@ def _one_device(**ts):
 
 
 def _no_grad(what, *ts):
+    if torch.jit.is_tracing():
+        raise RuntimeError("%s cannot be traced: the trace would hold its result as a constant" % what)
+    if _has_tangent(*ts):
+        raise RuntimeError("%s has no forward-mode gradient: call it on inputs without a tangent (torch.autograd.forward_ad)" % what)
     if torch.is_grad_enabled():
         for t in ts:
             if getattr(t, "requires_grad", False):
@@ -232,7 +237,7 @@ def quantize_rows(x, channels_first: bool = False) -> QuantizedRows:
 
 def quantize_rows_into(x, q, scale) -> None:
     """``quantize_rows`` of x [N, K] into q int8 [N, K] and scale float32 [N] that the caller owns."""
-    _no_grad("quantize_rows_into", x)
+    _no_grad("quantize_rows_into", x, scale)
     _check_quantize(x, False)
     _check_cache(q.unsqueeze(0), scale.unsqueeze(0), torch.empty(0, dtype=torch.int64), None)
     _one_device(x=x, q=q, scale=scale)

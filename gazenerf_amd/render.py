@@ -24,6 +24,7 @@ import os
 from typing import Dict, Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, _torch_ext
 
@@ -46,6 +47,13 @@ def params_to_list(params) -> list:
 
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else C.c_void_p(t.data_ptr())
+
+
+def _has_tangent(*ts) -> bool:
+    """Is one of the tensors a dual tensor of torch.autograd.forward_ad?  (``requires_grad`` says nothing about that.)"""
+    if getattr(forward_ad, "_current_level", 0) < 0:            # no dual level is open: nothing is dual
+        return False
+    return any(torch.is_tensor(t) and forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
 def _check_tensor(name, t, shape=None):

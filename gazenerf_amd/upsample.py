@@ -18,7 +18,7 @@ import torch
 from torch import nn
 
 from . import _lib
-from .render import _check_tensor, _stream_ptr
+from .render import _check_tensor, _has_tangent, _stream_ptr
 
 
 def renderer_param_names(n_blocks: int):
@@ -331,7 +331,7 @@ class NeuralRendererAMD(nn.Module):
             return self._render_int8(x)
         params = {k: v for k, v in self.named_parameters() if k != "bg_featmap"}
         if (self.graph_inference and not torch.is_grad_enabled() and x.is_cuda and x.dtype == torch.float32 and x.dim() == 4
-                and not torch.cuda.is_current_stream_capturing()):
+                and not torch.cuda.is_current_stream_capturing() and not _has_tangent(x, *params.values())):
             return self._graphed(x, params, self.n_blocks, self.min_feat, self.final_actvn)
         return neural_render(x, params, self.n_blocks, self.min_feat, self.final_actvn)
 

@@ -144,7 +144,7 @@ def neural_render_int8(x, params: Dict[str, torch.Tensor], n_blocks: int = 3, mi
     """``neural_render`` in 8 bits: x [B, feat_nc, S, S] -- or x None with a ``FeatureMapCache`` and int64 ``slots`` [B] on its device --
     -> image [B, 3, S*2^n, S*2^n].  ``weights`` keeps the quantised weights from call to call; a call that is being captured quantises them
     in the graph instead, so that a replay follows its parameters.  Inference only."""
-    int8._no_grad("neural_render_int8", x, *params.values())
+    int8._no_grad("neural_render_int8", x, getattr(cache, "scale", None), *params.values())
     dev = x if x is not None else getattr(cache, "q", None)
     if weights is None or (getattr(dev, "is_cuda", False) and torch.cuda.is_current_stream_capturing()):
         weights = Int8Weights()
@@ -168,6 +168,7 @@ class GraphedUpsample8:
         self.entries.clear()
 
     def __call__(self, params, n_blocks, min_feat, final_actvn, x=None, cache=None, slots=None):
+        int8._no_grad("neural_render_int8", x, getattr(cache, "scale", None), *params.values())
         with self.lock, self.weights.lock:
             return self._replay(params, n_blocks, min_feat, final_actvn, x, cache, slots)
 

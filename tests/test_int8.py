@@ -183,6 +183,26 @@ def test_no_backward(lib_built):
         G.int8_linear(x, w, torch.ones(5))
 
 
+def test_no_forward_mode_gradient_and_no_trace(lib_built):
+    """A tangent would be dropped (``requires_grad`` is False on a dual tensor), a trace would hold the result as a constant: both are refused."""
+    from torch.autograd import forward_ad
+    w, ones, slots = torch.zeros(5, 16, dtype=torch.int8), torch.ones(5), torch.zeros(1, dtype=torch.int64)
+    q, s = torch.zeros(1, 3, 16, dtype=torch.int8), torch.ones(1, 3)
+    params = {n: torch.zeros(1) for n in ("a", "b")}
+    calls = [lambda d: G.quantize_rows(d(torch.zeros(3, 16))), lambda d: G.int8_linear(d(torch.zeros(3, 16)), w, ones),
+             lambda d: G.int8_linear(torch.zeros(3, 16), w, d(ones)), lambda d: G.int8_linear(torch.zeros(3, 16), w, ones, d(torch.zeros(5))),
+             lambda d: G.int8_linear(q[0], w, ones, x_scale=d(s[0])), lambda d: G.write_featmaps(q, s, slots, d(torch.zeros(1, 16, 3))),
+             lambda d: G.write_featmaps(q, d(s), slots, torch.zeros(1, 16, 3)), lambda d: G.read_featmaps(q, d(s), slots),
+             lambda d: G.neural_render_int8(d(torch.zeros(1, 4, 16, 16)), params), lambda d: G.neural_render_int8(torch.zeros(1, 4, 16, 16), dict(params, b=d(ones)))]
+    for call in calls:
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), forward_ad.dual_level():
+                with pytest.raises(RuntimeError, match="no forward-mode gradient"):
+                    call(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
+    with torch.no_grad(), pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(lambda t: G.quantize_rows(t).scale, torch.zeros(3, 16), check_trace=False)
+
+
 def test_c_entries_refuse(lib_built):
     """The C ABI checks every size it indexes with before it launches anything (bogus pointers: nothing may be dereferenced)."""
     lib = _lib.load()

@@ -323,6 +323,25 @@ def test_module_copies():
 
 
 @gpu
+@pytest.mark.parametrize("precision", ["fp32", "int8"])
+def test_module_refuses_a_tangent(precision):
+    """A dual input or weight under no_grad, where a graph would be replayed: refused, not returned without its tangent."""
+    from torch.autograd import forward_ad
+    net = small_renderer(precision=precision)
+    x = features((1, 36, 16, 16), 1, 80).to(DEV)
+    with torch.no_grad():
+        want = net(x)
+        with forward_ad.dual_level():
+            with pytest.raises(RuntimeError, match="forward-mode gradient|forward mode AD"):
+                net(forward_ad.make_dual(x, torch.ones_like(x)))
+            assert torch.equal(net(x), want)
+            name, p = "feat_layers.0.weight", net.feat_layers[0].weight.detach()
+            with pytest.raises(RuntimeError, match="forward-mode gradient|forward mode AD"):
+                torch.func.functional_call(net, {name: forward_ad.make_dual(p, torch.ones_like(p))}, (x,))
+        assert torch.equal(net(x), want)
+
+
+@gpu
 def test_module_renders_cached_views():
     net = small_renderer()                                                       # fp32 by itself; cached views are 8-bit
     x = features((3, 36, 16, 16), 1, 9).to(DEV)
