@@ -148,16 +148,35 @@ def neural_render(x, params: Dict[str, torch.Tensor], n_blocks: int = 3, min_fea
     return _UpsampleFn.apply(cfg, x, *[params[n] for n in names])
 
 
-# Captures of this package run one at a time: torch.cuda.graph captures on ONE side stream that all threads share.  Other threads may go on
-# allocating and launching meanwhile (capture_error_mode="thread_local"; torch's own default forbids it to the whole process).
+# Captures of this package run one at a time, each device's on a stream of its own.  torch's streams come from a pool of 32 that it hands out
+# again and again, the one torch.cuda.graph captures on among them: work that another thread enqueues on "its" stream meanwhile would be
+# recorded instead of run.  Other threads may go on allocating (capture_error_mode="thread_local"; torch's default forbids it to all).
 _CAPTURE = threading.Lock()
+_CAPTURE_STREAMS: Dict[int, "torch.cuda.ExternalStream"] = {}
 
 
-def capture_graph(call):
-    """``call()`` recorded into a new ``torch.cuda.CUDAGraph`` on the current device."""
-    with _CAPTURE:
+def _capture_stream(dev):
+    """The device's capture stream (default priority), made on first use and kept; the caller holds ``_CAPTURE``."""
+    index = dev.index if dev.index is not None else torch.cuda.current_device()
+    if index not in _CAPTURE_STREAMS:
+        handle = C.c_void_p()
+        rc = _lib.load().hipStreamCreateWithFlags(C.byref(handle), C.c_uint(1))        # the runtime libgnr is linked to; 1: hipStreamNonBlocking
+        if rc:
+            raise RuntimeError("hipStreamCreateWithFlags returned %d" % rc)
+        _CAPTURE_STREAMS[index] = torch.cuda.ExternalStream(handle.value, device=index)
+    return _CAPTURE_STREAMS[index]
+
+
+def capture_graph(dev, call):
+    """``call()`` -- run once outside the capture (module load, argument errors), then recorded into a new ``torch.cuda.CUDAGraph``."""
+    with _CAPTURE, torch.cuda.device(dev):
+        stream, current = _capture_stream(dev), torch.cuda.current_stream(dev)
+        stream.wait_stream(current)
+        with torch.cuda.stream(stream):
+            call()
+        current.wait_stream(stream)
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+        with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
             call()
     return graph
 
@@ -242,12 +261,7 @@ class GraphedUpsample:
             def call():
                 _lib.check(lib.gnr_upsample_fwd(C.byref(p), C.byref(w), C.c_void_p(img.data_ptr()), C.c_void_p(ws.data_ptr()),
                                                 ws.numel(), _stream_ptr(dev)), lib)
-            side = torch.cuda.Stream(device=dev)
-            side.wait_stream(torch.cuda.current_stream(dev))
-            with torch.cuda.stream(side):
-                call()                                  # warm-up outside the capture (module load, argument errors)
-            torch.cuda.current_stream(dev).wait_stream(side)
-            graph = capture_graph(call)
+            graph = capture_graph(dev, call)
         self.captures += 1
         return graph, x_static, img, ws, params, p, w      # the graph's kernels point into all of these: keep them alive
 

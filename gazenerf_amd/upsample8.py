@@ -202,14 +202,7 @@ class GraphedUpsample8:
         for n, t in call.params.items():
             if t.data_ptr() != params[n].data_ptr():
                 raise ValueError("GraphedUpsample8: parameter %s is not contiguous; the graph would read a temporary copy" % n)
-        dev = given.device
-        with torch.cuda.device(dev):
-            side = torch.cuda.Stream(device=dev)
-            side.wait_stream(torch.cuda.current_stream(dev))
-            with torch.cuda.stream(side):
-                call()                                               # warm-up outside the capture
-            torch.cuda.current_stream(dev).wait_stream(side)
-            graph = capture_graph(call)
+        graph = capture_graph(given.device, call)
         self.captures += 1
         return graph, static, call
 

@@ -481,3 +481,16 @@ def test_graph_replays_on_two_streams_share_no_buffer(threads):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in got)
     assert net._graphed.captures == 2
+
+
+@pytest.mark.gpu
+def test_graphs_are_captured_on_a_stream_nobody_else_gets():
+    """torch hands its 32 streams out again and again.  A capture on one of them would record what another thread enqueues on "its" stream
+    meanwhile: the capture stream is not among them, and captures use it alone."""
+    from gazenerf_amd import upsample
+    dev = _dev()
+    seen = []
+    upsample.capture_graph(dev, lambda: seen.append(torch.cuda.current_stream(dev).cuda_stream))
+    own = upsample._CAPTURE_STREAMS[dev.index or 0].cuda_stream
+    assert seen == [own, own]
+    assert own not in {torch.cuda.Stream().cuda_stream for _ in range(200)} | {torch.cuda.default_stream().cuda_stream}
