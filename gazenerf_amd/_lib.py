@@ -146,7 +146,7 @@ def check_build_info(info: str, path: str):
     want = source_hash()
     if want is not None and bi["src"] != want:
         raise RuntimeError(
-            "gazenerf_amd: %s was built from other sources than this tree (library src=%s, tree src=%s): rebuild with "
+            "gazenerf_amd: %s was built from other sources or compiler options than this tree (library src=%s, tree src=%s): rebuild with "
             "`python -m gazenerf_amd.build`" % (path, bi["src"], want))
     if bi["experimental"] != "0" or bi["flags"]:
         if os.environ.get("GNR_ALLOW_EXPERIMENTAL_LIB", "") != "1":

@@ -1,4 +1,5 @@
-"""Hash of the sources libgnr.so / _gnr_torch.so are built from (csrc/*.hip, *.h, *.cpp and include/gnr.h).
+"""Hash of what libgnr.so / _gnr_torch.so are built from: the sources (csrc/*.hip, *.h, *.cpp and include/gnr.h) and the
+compiler options of ``gazenerf_amd.build``, which change the kernels' arithmetic as well as a source does.
 
 ``gazenerf_amd.build`` compiles it into the library (``gnr_build_info()``); ``_lib.load()`` recomputes it from the tree and
 refuses a library built from other sources -- the binaries are git-ignored and travel to the GPU box prebuilt, so without
@@ -22,7 +23,9 @@ def source_hash():
     """16 hex digits, or None when the tree carries no sources (an installed copy: nothing to compare with)."""
     if not os.path.isdir(CSRC) or not os.path.exists(HEADER):
         return None
+    from . import build
     h = hashlib.sha256()
+    h.update(repr((build.FLAGS, sorted(build.EXTRA_FLAGS.items()))).encode() + b"\0")
     for path in source_files():
         h.update(os.path.basename(path).encode() + b"\0")
         with open(path, "rb") as f:

@@ -41,9 +41,22 @@ def _stale(target, deps):
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
+def _options(source: str):
+    """hipcc's options for one file of SOURCES, without the ones of a timing experiment."""
+    return FLAGS + EXTRA_FLAGS.get(source, [])
+
+
+def _other_options(obj: str, source: str) -> bool:
+    """Was `obj` compiled with other options than today's (or before they were recorded beside it)?"""
+    try:
+        return open(obj + ".opts").read() != repr(_options(source))
+    except OSError:
+        return True
+
+
 def build_info_string() -> str:
-    """What gnr_build_info() of the library being built returns: `src=<hash of csrc/ + include/gnr.h>;flags=<extra -D
-    switches, with the files they were applied to>;experimental=<0|1>`."""
+    """What gnr_build_info() of the library being built returns: `src=<hash of csrc/ + include/gnr.h + the options
+    above>;flags=<extra -D switches, with the files they were applied to>;experimental=<0|1>`."""
     from ._srchash import source_hash
     flags = ""
     if EXPERIMENT_FLAGS:
@@ -64,13 +77,13 @@ def build(force: bool = False, verbose: bool = True) -> str:
         obj = os.path.join(OBJ, s.replace(".hip", ".o"))
         # gnr_api.hip carries the build-info string: recompiled whenever any source (or the flag list) changed; after
         # an experimental build every object is suspect
-        if (force or s in EXPERIMENT_FILES or was_experimental or _stale(obj, [src] + hdrs)
+        if (force or s in EXPERIMENT_FILES or was_experimental or _stale(obj, [src] + hdrs) or _other_options(obj, s)
                 or (s == "gnr_api.hip" and info != old_info)):
             jobs.append((src, obj))
 
     def compile_one(job):
         src, obj = job
-        cmd = [HIPCC] + FLAGS + EXTRA_FLAGS.get(os.path.basename(src), [])
+        cmd = [HIPCC] + _options(os.path.basename(src))
         if os.path.basename(src) in EXPERIMENT_FILES:
             cmd += EXPERIMENT_FLAGS
         if EXPERIMENT_FLAGS:
@@ -83,6 +96,8 @@ def build(force: bool = False, verbose: bool = True) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("hipcc failed for %s:\n%s\n%s" % (src, r.stdout, r.stderr))
+        with open(obj + ".opts", "w") as f:
+            f.write(repr(_options(os.path.basename(src))))
         return r.stderr
 
     with ThreadPoolExecutor(max_workers=max(1, min(len(jobs), os.cpu_count() or 1))) as ex:

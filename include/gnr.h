@@ -414,10 +414,10 @@ int gnr_upsample_int8_fwd(const GnrUpsampleProblem* p, const GnrUpsampleWeights*
 
 const char* gnr_last_error(void);
 
-/* ABI 4.  What this binary was built from: "src=<16 hex digits: sha256 over gazenerf_amd/csrc/{*.hip,*.h,*.cpp} and this
- * header, in name order>;flags=<extra -D switches of a timing-experiment build, with the files they applied to>;
+/* ABI 4.  What this binary was built from: "src=<16 hex digits: sha256 over the compiler options, gazenerf_amd/csrc/
+ * {*.hip,*.h,*.cpp} in name order and this header>;flags=<extra -D switches of a timing-experiment build, with the files they applied to>;
  * experimental=<0|1>".  The binaries are not under version control (they travel to the GPU box prebuilt): a binding
- * recomputes the hash from the tree it runs in and refuses a library built from other sources, or an experimental build
+ * recomputes the hash from the tree it runs in and refuses a library built from other sources or options, or an experimental build
  * (gazenerf_amd/_lib.py does both).  Timing switches that change results only compile with -DGNR_EXPERIMENTAL_BUILD
  * (gazenerf_amd/csrc/gnr_internal.h), which `python -m gazenerf_amd.build` adds -- and reports here -- whenever extra flags
  * are given. */

@@ -253,3 +253,48 @@ def test_the_guard_band_allocator_builds_and_exports_its_hooks():
     for name in os.listdir(pkg):
         if name.endswith(".py") and name != "build.py":
             assert "guard_alloc" not in open(os.path.join(pkg, name)).read(), name
+
+
+def test_a_change_of_compiler_options_rebuilds_and_is_refused(tmp_path, monkeypatch):
+    """The options belong to what a binary is built from: with others the hash differs (so a library built with the old ones is refused)
+    and the objects they apply to are compiled again.  hipcc is replaced by a stand-in that only writes its output file."""
+    import pytest
+    from gazenerf_amd import _lib, _srchash, build
+    monkeypatch.delenv("GNR_ALLOW_EXPERIMENTAL_LIB", raising=False)
+    monkeypatch.setattr(build, "OBJ", str(tmp_path))
+    monkeypatch.setattr(build, "STAMP", str(tmp_path / "build_info.txt"))
+    monkeypatch.setattr(build, "LIB", str(tmp_path / "libgnr.so"))
+    compiled = []
+
+    class Done:
+        returncode, stdout, stderr = 0, "", ""
+
+    def run(cmd, **kw):
+        if "-c" in cmd:
+            compiled.append(os.path.basename(cmd[cmd.index("-c") + 1]))
+        open(cmd[cmd.index("-o") + 1], "w").close()
+        return Done()
+
+    monkeypatch.setattr(build.subprocess, "run", run)
+
+    def rebuilt():
+        compiled.clear()
+        build.build(verbose=False)
+        return sorted(compiled)
+
+    assert rebuilt() == sorted(build.SOURCES)
+    assert rebuilt() == []
+    was = build.build_info_string()
+    _lib.check_build_info(was, "libgnr.so")
+    monkeypatch.setattr(build, "FLAGS", build.FLAGS + ["-DX=1"])
+    assert build.build_info_string() != was
+    with pytest.raises(RuntimeError, match="compiler options"):
+        _lib.check_build_info(was, "libgnr.so")
+    assert rebuilt() == sorted(build.SOURCES) and rebuilt() == []
+    was = _srchash.source_hash()
+    monkeypatch.setattr(build, "EXTRA_FLAGS", {"gnr_prep.hip": ["-DY=1"]})
+    assert _srchash.source_hash() != was
+    again = rebuilt()                                        # the file that gained an option, the one that lost it, and the one with the hash
+    assert again == ["gnr_api.hip", "gnr_prep.hip", "gnr_wgrad.hip"] and rebuilt() == []
+    os.remove(str(tmp_path / "gnr_vd.o.opts"))               # an object from before the options were recorded
+    assert rebuilt() == ["gnr_vd.hip"]
