@@ -87,8 +87,10 @@ template <bool FAR> __device__ __forceinline__ fv4 scaled(fv4 sum, fv4 sx, fv4 s
 // 4 KiB blocks a wave.  (Workgroups that walk several tiles and request the next one's stages under the epilogue were built: they need
 // twice the registers, and 262144 x 64 -> 32 took 9.2 us against 8.5, 458752 x 128 -> 256 64 against 56.)
 // ---------------------------------------------------------------------------------------------
+// m0 holds the LDS address; the compiler may keep a value of its own there and takes no clobber for it (a reserved register): it is put back
 __device__ __forceinline__ void dma16(const int8_t* p, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory");
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(p), "s"(lds) : "memory");
 }
 template <int N> __device__ __forceinline__ void wait_vm() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N < 63 ? N : 63) : "memory");     // six bits; fewer than allowed is only stricter

@@ -762,3 +762,19 @@ def test_under_guard_bands(binding, poison):
     d = _guarded("int8", "--binding", binding, "--cases", "25", "--seed", "7" if poison else "8", *(["--poison"] if poison else []))
     assert d["ok"] and d["violations"] == 0, (d["report"], d["cases"])
     assert d["calls_checked"] >= 25 * 6
+
+
+def test_m0_is_put_back():
+    """Inline assembly that writes m0 (a reserved register: the compiler takes no clobber for it) saves it first and restores it last."""
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(os.path.abspath(G.__file__)), "csrc")
+    found = 0
+    for name in ("gnr_int8.hip", "gnr_int8.h", "gnr_quant.hip", "gnr_upsample8.hip"):
+        text = open(os.path.join(csrc, name)).read()
+        for block in re.findall(r'asm\s+volatile\s*\(\s*"([^"]*)"', text):
+            steps = block.split("\\n\\t")
+            if any(re.match(r"s_mov_b32 m0,", s) for s in steps):
+                found += 1
+                assert re.match(r"s_mov_b32 %0, m0$", steps[0]) and re.match(r"s_mov_b32 m0, %0$", steps[-1]), (name, block)
+    assert found
