@@ -475,6 +475,12 @@ Tensor int8_linear(const Tensor& x, const Tensor& w_q, const Tensor& w_scale, co
         } else {
             TORCH_CHECK(x.dim() >= 1, "rows must be [..., K]");
             xr = rows_in(x);
+            // entries that stand one behind the other are one: which kernel takes them goes by their number, not by how they are counted
+            if (xr.b > 1 && (xr.n == 1 || xr.sb == xr.n * xr.sn)) {
+                if (xr.n == 1) xr.sn = xr.sb;
+                xr.n *= xr.b;
+                xr.b = 1;
+            }
         }
         b = xr.b; n = xr.n;
         TORCH_CHECK(xr.k == k, "x has another number of channels than w_q: ", x.sizes(), ", ", w_q.sizes());

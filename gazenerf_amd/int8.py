@@ -173,6 +173,15 @@ def _rows3(t):
     return t if t.stride(2) == 1 or k == 1 else t.contiguous()
 
 
+def _one_entry(t):
+    """Rows [b, n, K] as [1, b n, K] where the entries stand one behind the other: which kernel takes them goes by their number, not by how
+    they are counted."""
+    b, n, k = t.shape
+    if b <= 1 or n < 1 or not (n == 1 or t.stride(0) == n * t.stride(1)):
+        return t
+    return t.as_strided((1, b * n, k), (0, t.stride(0) if n == 1 else t.stride(1), t.stride(2)))
+
+
 def _pitched(q):
     """8-bit rows [b, n, K] as a product reads them: on 16-byte boundaries, readable to the next multiple of 16."""
     b, n, k = q.shape
@@ -376,7 +385,7 @@ def int8_linear(x, w_q, w_scale, bias=None, *, x_scale=None, slots=None, leaky: 
         shape = (b, o) + tuple(x.shape[2:])
         keep.append(xr)
     else:
-        xr = _rows3(x)
+        xr = _one_entry(_rows3(x))
         b, n = xr.shape[:2]
         p.x_batch, p.x_stride = int(xr.stride(0)), int(xr.stride(1))
         shape = tuple(x.shape[:-1]) + (o,)

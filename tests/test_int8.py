@@ -571,6 +571,42 @@ def test_linear_shapes_strides_and_empties():
         G.int8_linear(xd, wq.q.cpu(), wq.scale)
 
 
+def test_rows_of_three_dimensions_are_one_entry():
+    """The ctypes binding's view of floating rows [b, n, K]: one entry where they stand one behind the other, the same values always."""
+    x = torch.arange(4 * 6 * 5.0).reshape(4, 6, 5)
+    for t, one in ((x, True), (x[:, :1], True), (x[:1], False), (x[:, :5], False), (x[:, ::2], True), (x[::2], False), (x[:, :0], False), (x[:, 2:3].expand(4, 3, 5), False)):
+        y = int8._one_entry(t)
+        assert torch.equal(y.reshape(-1, 5), t.reshape(-1, 5)) and (y.shape[0] == 1 and t.shape[0] > 1) == one, t.shape
+
+
+@gpu
+@pytest.mark.parametrize("binding", ["auto", "ctypes"])
+@pytest.mark.parametrize("k", [40, 517])
+def test_linear_rows_of_three_dimensions(k, binding, monkeypatch):
+    """The same bits however the rows are counted, and no workspace for [4, 4, K] where [16, K] needs none."""
+    if binding == "ctypes":
+        monkeypatch.setattr(_torch_ext, "active", lambda: None)
+    w, b = weights(33, k, 3)
+    wq, bd = G.quantize_rows(w.to(DEV)), b.to(DEV)
+    for shape in ((4, 4, k), (16, 1, k), (1, 16, k), (5, 130, k)):
+        x = features(shape, 2, 5).to(DEV)
+        want = G.int8_linear(x.reshape(-1, k), wq.q, wq.scale, bd, leaky=True).reshape(shape[:2] + (33,))
+        apart = torch.zeros(shape[0], shape[1] + 2, k, device=DEV)
+        apart[:, :shape[1]] = x
+        for y in (x, x.transpose(0, 1).contiguous().transpose(0, 1), apart[:, :shape[1]], apart[:, :shape[1]].contiguous()):
+            assert torch.equal(G.int8_linear(y, wq.q, wq.scale, bd, leaky=True), want)
+
+    def largest(x):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        G.int8_linear(x, wq.q, wq.scale, bd)
+        return torch.cuda.max_memory_allocated() - before
+
+    x = features((16, k), 1, 6).to(DEV)
+    assert largest(x.reshape(4, 4, k)) == largest(x) < largest(torch.zeros(4, 5, k, device=DEV)[:, :4])
+
+
 @gpu
 def test_linear_special_values():
     """Zero rows give act(bias); a row with Inf / NaN gives NaN and leaves its neighbours alone; fp16 outputs overflow to Inf."""
