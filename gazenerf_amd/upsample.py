@@ -181,6 +181,43 @@ def capture_graph(dev, call):
     return graph
 
 
+class RecentlyUsed:
+    """At most ``most`` values by key.  A new key takes the place of the one used longest ago, but only if that was not used in the last
+    ``8 * most`` lookups: keys that are used in turn, more of them than places, would otherwise replace each other for ever -- and each
+    replacement captures a graph, a thousand times the price of a call without one.  Values are dropped while nothing is captured: the end
+    of a graph waits for the device."""
+
+    def __init__(self, most: int):
+        self.most, self.lookups, self.values, self.used = most, 0, {}, {}
+
+    def __len__(self):
+        return len(self.values)
+
+    def get(self, key):
+        self.lookups += 1
+        if key in self.values:
+            self.used[key] = self.lookups
+        return self.values.get(key)
+
+    def room(self) -> bool:
+        """May ``put`` be called for a new key?  Makes room where it may."""
+        if len(self.values) >= self.most:
+            oldest = min(self.used, key=self.used.get)
+            if self.lookups - self.used[oldest] <= 8 * self.most:
+                return False
+            with _CAPTURE:
+                del self.values[oldest], self.used[oldest]
+        return True
+
+    def put(self, key, value):
+        self.values[key], self.used[key] = value, self.lookups
+
+    def clear(self):
+        with _CAPTURE:
+            self.values.clear()
+            self.used.clear()
+
+
 class GraphedUpsample:
     """Inference forward of the upsampler replayed from a HIP graph (round 4).
 
@@ -192,17 +229,19 @@ class GraphedUpsample:
     static image.  The weight re-layout
     (``conv16_pack_kernel``) is INSIDE the graph, so in-place parameter updates are seen by the next replay; a parameter
     that moves to other storage (``.to()``, ``load_state_dict`` into new tensors, ``p.data = ...``) changes the key and the
-    forward is captured again.  Inference only: nothing is saved for a backward."""
+    forward is captured again.  Where there are more of them in use than ``max_entries``, the others run without a graph.
+    Inference only: nothing is saved for a backward."""
 
     def __init__(self, max_entries: int = 8):
-        self.entries = {}
+        self.entries = RecentlyUsed(max_entries)
         self.max_entries = max_entries
         self.lock = threading.Lock()
         self.captures = 0
         self.replays = 0
 
     def clear(self):
-        self.entries.clear()
+        with self.lock:
+            self.entries.clear()
 
     # the cache holds CUDAGraph objects and ctypes structs of device pointers: a copy / pickle of the owning module starts
     # with an empty cache (and captures again on its first inference call)
@@ -223,16 +262,16 @@ class GraphedUpsample:
             tuple(tuple(t.shape) for t in flat)
         with self.lock:
             ent = self.entries.get(key)
-            if ent is None:
+            if ent is None and self.entries.room():
                 ent = self._capture(x, flat, dict(n_blocks=int(n_blocks), min_feat=int(min_feat), final_actvn=bool(final_actvn)))
-                if len(self.entries) >= self.max_entries:
-                    self.entries.pop(next(iter(self.entries)))
-                self.entries[key] = ent
-            graph, x_static, img_static = ent[:3]
-            x_static.copy_(x)
-            graph.replay()
-            self.replays += 1
-            return img_static.clone() if copy_output else img_static
+                self.entries.put(key, ent)
+            if ent is not None:
+                graph, x_static, img_static = ent[:3]
+                x_static.copy_(x)
+                graph.replay()
+                self.replays += 1
+                return img_static.clone() if copy_output else img_static
+        return neural_render(x, params, n_blocks, min_feat, final_actvn)
 
     def _capture(self, x, flat, cfg):
         lib = _lib.load()
@@ -327,9 +366,10 @@ class NeuralRendererAMD(nn.Module):
         params = {k: v for k, v in self.named_parameters() if k != "bg_featmap"}
         dev = x if x is not None else cache.q
         capturing = dev.is_cuda and torch.cuda.is_current_stream_capturing()
-        if self.graph_inference and not torch.is_grad_enabled() and dev.is_cuda and not capturing:
-            return self._int8(dev.device)(params, self.n_blocks, self.min_feat, self.final_actvn, x, cache, slots)
-        weights = None if capturing else self._int8(dev.device).weights
+        renderer = None if capturing else self._int8(dev.device)
+        if renderer is not None and self.graph_inference and not torch.is_grad_enabled() and dev.is_cuda:
+            return renderer(params, self.n_blocks, self.min_feat, self.final_actvn, x, cache, slots)
+        weights = None if renderer is None else renderer.weights
         return neural_render_int8(x, params, self.n_blocks, self.min_feat, self.final_actvn, weights, cache, slots)
 
     def render_cached(self, cache, slots):

@@ -15,7 +15,7 @@ import torch
 
 from . import _lib, int8
 from .render import _check_tensor, _stream_ptr
-from .upsample import _expected_shapes, _weights_struct, capture_graph, renderer_param_names
+from .upsample import RecentlyUsed, _expected_shapes, _weights_struct, capture_graph, renderer_param_names
 
 _CONVS = (("up1", "feat_upsample_list.%d.layer_1"), ("up2", "feat_upsample_list.%d.layer_2"), ("feat", "feat_layers.%d"))
 
@@ -156,16 +156,17 @@ class GraphedUpsample8:
     some thirty launches of a few microseconds.  The graph reads the quantised weights of ``weights``, refreshed before each replay if a
     parameter changed, and the biases and RGB weights in place; the input (a map, or the slots) is copied into the graph's own buffer.
     For one HIP stream, from any number of threads: between a call's copy into that buffer and its copy out of the image nobody else's
-    work is enqueued."""
+    work is enqueued.  Where there are more shapes and caches in use than ``max_entries``, the others run without a graph."""
 
     def __init__(self, weights: Int8Weights, max_entries: int = 4):
         self.weights, self.max_entries = weights, max_entries
         self.lock = threading.Lock()
-        self.entries = {}
+        self.entries = RecentlyUsed(max_entries)
         self.captures = self.replays = 0
 
     def clear(self):
-        self.entries.clear()
+        with self.lock:
+            self.entries.clear()
 
     def __call__(self, params, n_blocks, min_feat, final_actvn, x=None, cache=None, slots=None):
         int8._no_grad("neural_render_int8", x, getattr(cache, "scale", None), *params.values())
@@ -181,11 +182,11 @@ class GraphedUpsample8:
             key += (cache.q.data_ptr(), cache.scale.data_ptr(), tuple(cache.q.shape), cache.q.stride(), cache.scale.stride())
         ent = self.entries.get(key)
         if ent is None:
+            if not self.entries.room():
+                return _Call(params, self.weights, n_blocks, min_feat, final_actvn, x, cache, slots)()
             with torch.inference_mode(False), torch.no_grad():       # the static buffers outlive this call
                 ent = self._capture(params, n_blocks, min_feat, final_actvn, x, cache, slots)
-            if len(self.entries) >= self.max_entries:
-                self.entries.pop(next(iter(self.entries)))
-            self.entries[key] = ent
+            self.entries.put(key, ent)
         graph, static, call = ent
         static.copy_(given)
         graph.replay()
@@ -208,29 +209,28 @@ class GraphedUpsample8:
 
 
 class Int8Renderers:
-    """A ``GraphedUpsample8`` (with its ``Int8Weights``) per HIP stream: what two streams run at once shares no buffer.  The
-    ``max_streams`` used last are kept.  A copy starts empty: graphs and structs of device pointers are not copied."""
+    """A ``GraphedUpsample8`` (with its ``Int8Weights``) per HIP stream: what two streams run at once shares no buffer.  Where there are more
+    streams in use than ``max_streams``, the others get None: they run without a graph and quantise the weights in every call.  A copy
+    starts empty: graphs and structs of device pointers are not copied."""
 
     def __init__(self, max_streams: int = 4):
         self.max_streams = max_streams
-        self.streams = {}
+        self.streams = RecentlyUsed(max_streams)
         self.lock = threading.Lock()
 
-    def __call__(self, dev) -> GraphedUpsample8:
-        key = torch.cuda.current_stream(dev).cuda_stream if dev.type == "cuda" else None
+    def __call__(self, dev) -> Optional[GraphedUpsample8]:
+        key = (dev, torch.cuda.current_stream(dev).cuda_stream if dev.type == "cuda" else None)
         with self.lock:
-            r = self.streams.pop((dev, key), None)
-            if r is None:
+            r = self.streams.get(key)
+            if r is None and self.streams.room():
                 r = GraphedUpsample8(Int8Weights())
-                while len(self.streams) >= self.max_streams:
-                    self.streams.pop(next(iter(self.streams)))
-            self.streams[dev, key] = r
+                self.streams.put(key, r)
         return r
 
     def look_again(self):
         """The next call on each stream quantises its weights again."""
         with self.lock:
-            for r in self.streams.values():
+            for r in self.streams.values.values():
                 with r.weights.lock:
                     r.weights.seen = None
 

@@ -494,3 +494,18 @@ def test_graphs_are_captured_on_a_stream_nobody_else_gets():
     own = upsample._CAPTURE_STREAMS[dev.index or 0].cuda_stream
     assert seen == [own, own]
     assert own not in {torch.cuda.Stream().cuda_stream for _ in range(200)} | {torch.cuda.default_stream().cuda_stream}
+
+
+@pytest.mark.gpu
+def test_more_shapes_than_graphs_run_without_one():
+    """Ten batch sizes in turn with eight places: eight graphs, captured once; the others run eagerly and give the same bits."""
+    from gazenerf_amd import NeuralRendererAMD
+    dev = _dev()
+    torch.manual_seed(0)
+    net = NeuralRendererAMD(feat_nc=64, featmap_size=16, img_size=32, min_feat=16).to(dev).eval()
+    xs = [synth.synth_featmap(b, 64, 16, seed=b).to(dev) for b in range(1, 11)]
+    want = [neural_render_eager(net, x).detach() for x in xs]
+    with torch.no_grad():
+        for _ in range(3):
+            assert all(torch.equal(net(x), w) for x, w in zip(xs, want))
+    assert net._graphed.captures == 8 and net._graphed.replays == 24

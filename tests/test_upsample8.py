@@ -254,6 +254,60 @@ def test_weights_copy_empty():
         assert not twin.rows and twin.seen is None and twin.quantised == 0 and twin.lock is not w.lock
 
 
+def test_more_streams_than_renderers(monkeypatch):
+    """Streams used in turn keep what they have: the fifth of five gets none, instead of taking the place of one that is about to come back.
+    A stream that is not used any more makes room in the end."""
+    now = type("Stream", (), {})()
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda dev=None: now)
+    renderers, dev = upsample8.Int8Renderers(), torch.device("cuda", 0)
+
+    def on(handle):
+        now.cuda_stream = handle
+        return renderers(dev)
+    first = [on(h) for h in range(5)]
+    assert all(r is not None for r in first[:4]) and len(set(map(id, first))) == 5 and first[4] is None
+    for _ in range(20):
+        assert [on(h) for h in range(5)] == first
+    assert [on(4) for _ in range(40)][-1] is not None and len(renderers.streams) == 4     # the other four fell silent
+    assert sum(on(h) is None for h in range(5)) == 1
+
+
+@gpu
+def test_module_on_more_streams_than_it_keeps_graphs_for():
+    """Six streams in turn: four graphs, captured once; the images are right on all of them, after a change of the weights too."""
+    net = small_renderer(precision="int8")
+    x = features((1, 36, 16, 16), 1, 90).to(DEV)
+    params = {k: v for k, v in net.named_parameters() if k != "bg_featmap"}
+    streams = [torch.cuda.Stream() for _ in range(6)]
+    with torch.no_grad():
+        for turn in range(4):
+            want = G.neural_render_int8(x, params, 2, 8)
+            torch.cuda.synchronize()
+            got = []
+            for s in streams:
+                with torch.cuda.stream(s):
+                    got.append(net(x))
+            torch.cuda.synchronize()
+            assert all(torch.equal(g, want) for g in got)
+            net.feat_layers[0].weight.mul_(1.25)
+            torch.cuda.synchronize()
+    kept = list(net._int8.streams.values.values())
+    assert len(kept) == 4 and all(r.captures == 1 and r.replays == 4 and r.weights.quantised == 4 for r in kept)
+
+
+@gpu
+def test_more_batch_sizes_than_graphs():
+    net = small_renderer(precision="int8")
+    xs = [features((b, 36, 16, 16), 1, b).to(DEV) for b in range(1, 7)]
+    params = {k: v for k, v in net.named_parameters() if k != "bg_featmap"}
+    with torch.no_grad():
+        want = [G.neural_render_int8(x, params, 2, 8) for x in xs]
+        for _ in range(3):
+            assert all(torch.equal(net(x), w) for x, w in zip(xs, want))
+    graphed = net._int8(torch.device(DEV, torch.cuda.current_device()))
+    assert graphed.captures == 4 and graphed.replays == 12 and graphed.weights.quantised == 1
+
+
 @gpu
 @pytest.mark.parametrize("own_streams", [False, True])
 def test_module_in_threads(own_streams):
