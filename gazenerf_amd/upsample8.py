@@ -203,7 +203,11 @@ class GraphedUpsample8:
         for n, t in call.params.items():
             if t.data_ptr() != params[n].data_ptr():
                 raise ValueError("GraphedUpsample8: parameter %s is not contiguous; the graph would read a temporary copy" % n)
+        if x is None and call.scale.data_ptr() != cache.scale.data_ptr():
+            raise ValueError("GraphedUpsample8: the cache's scales are not contiguous; the graph would read a temporary copy")
         graph = capture_graph(given.device, call)
+        if x is None:
+            call.q = call.scale = None       # the caller's: the key holds their addresses, so a replay's caller has them, and a dropped cache is free
         self.captures += 1
         return graph, static, call
 

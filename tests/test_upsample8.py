@@ -309,6 +309,25 @@ def test_more_batch_sizes_than_graphs():
 
 
 @gpu
+def test_a_graph_does_not_keep_a_cache():
+    """A deleted FeatureMapCache gives its memory back, although a graph that read it is still there."""
+    net = small_renderer()
+    x = features((2, 36, 16, 16), 1, 91).to(DEV)
+    cache = G.FeatureMapCache(2000, 36, 256, device=DEV)
+    cache.write([0, 1], x)
+    with torch.no_grad():
+        want = net.render_cached(cache, [1, 0])
+    torch.cuda.synchronize()
+    held, size = torch.cuda.memory_allocated(), cache.q.untyped_storage().nbytes() + cache.scale.untyped_storage().nbytes()
+    del cache
+    assert held - torch.cuda.memory_allocated() >= size
+    again = G.FeatureMapCache(2000, 36, 256, device=DEV)                          # likely where the first one stood: the graph reads it in place
+    again.write([0, 1], x.flip(0))
+    with torch.no_grad():
+        assert torch.equal(net.render_cached(again, [0, 1]), want)
+
+
+@gpu
 @pytest.mark.parametrize("own_streams", [False, True])
 def test_module_in_threads(own_streams):
     """Three threads, each with its own map, on the default stream and on streams of their own; the graphs are captured while the others run."""
