@@ -82,22 +82,27 @@ struct CompBwdParams {
     int accumulate;
 };
 
-constexpr int CB_MAX = 512;
+// Accumulated in 64 bits: q_i and the weighted mean of the q_j behind it nearly cancel where the density head saturates, and a sum of the
+// terms' gradients cancels once more (density bias: |sum| down to 1/36 of the sum of magnitudes).  In fp32 the rounding of q, of the suffix sums
+// and of S / x was 3-10 x the rest of the pass's error there.  The kernel waits for memory: same time.  What less than CB_LEAST of a ray's light
+// reaches (1e-24; in fp32 the products below 1e-38 vanished) counts as 0: it would only leave gradients under fp32's normal range behind,
+// which are not linear in the upstream gradient any more.
+constexpr double CB_LEAST = 0x1p-80;
+constexpr size_t cb_lds(int np) { return sizeof(double) * (4 * 4 * (size_t)np + 4 * FEAT_PAD); }       // q, x, T, S and g of four rays
 
 __global__ __launch_bounds__(256) void comp_bwd_kernel(const CompBwdParams cp) {
-    __shared__ float sh_q[4][CB_MAX], sh_x[4][CB_MAX], sh_T[4][CB_MAX], sh_S[4][CB_MAX], sh_g[4][FEAT_PAD];
+    extern __shared__ double cb_smem[];
     const GnrProblem& p = cp.prob;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long n_rays_total = (long)p.batch * p.n_rays;
     const long ray = (long)blockIdx.x * 4 + wave;
     const bool live = ray < n_rays_total;
     const int np = p.n_samples, cpr = cp.chunks_per_ray;
-    float* q = sh_q[wave]; float* xx = sh_x[wave]; float* TT = sh_T[wave]; float* SS = sh_S[wave];
+    double *q = cb_smem + wave * (4 * np + FEAT_PAD), *xx = q + np, *TT = xx + np, *SS = TT + np, *gsh = SS + np;
     const long row0 = live ? ray * cpr * CHUNK : 0;       // padded rows of this ray are contiguous
 
     // q_i = g . feat_i - g_bg: the features are CCM ([chunk][288][32]), so a lane owns one sample and
     // walks the channels; each load instruction covers two full 128-byte rows (two chunks).
-    float* gsh = sh_g[wave];
     if (live)
         for (int c = lane; c < FEAT_PAD; c += 64) gsh[c] = cp.gT[ray * FEAT_PAD + c];
     const float gbg = (live && cp.g_bg) ? cp.g_bg[ray] : 0.0f;
@@ -107,7 +112,7 @@ __global__ __launch_bounds__(256) void comp_bwd_kernel(const CompBwdParams cp) {
             const float* fr = cp.act_feat + (row0 / CHUNK + i / CHUNK) * (long)(CHUNK * FEAT_PAD) + (i % CHUNK);
             // 16 loads in flight per lane (round 3; 4 before: 16 waves x 1 KiB per CU did not cover the HBM latency --
             // 0.68 of the 8 TB/s spec); four accumulator chains as before, so the summation order is unchanged
-            float v0 = 0.0f, v1 = 0.0f, v2 = 0.0f, v3 = 0.0f;
+            double v0 = 0.0, v1 = 0.0, v2 = 0.0, v3 = 0.0;
             static_assert(FEAT_PAD % 16 == 0, "unroll");
             // round 5: only the 16-channel groups that hold real channels (258 -> 272 of the layout's 288; the upstream
             // gradient of a padded channel is zero, so the skipped terms were fmaf(f, 0, v) = v: same bits, 5.6 % fewer bytes)
@@ -118,10 +123,10 @@ __global__ __launch_bounds__(256) void comp_bwd_kernel(const CompBwdParams cp) {
                 for (int u = 0; u < 16; ++u) f[u] = __builtin_nontemporal_load(fr + (n + u) * CHUNK);
 #pragma unroll
                 for (int u = 0; u < 16; u += 4) {
-                    v0 = fmaf(f[u + 0], gsh[n + u + 0], v0);
-                    v1 = fmaf(f[u + 1], gsh[n + u + 1], v1);
-                    v2 = fmaf(f[u + 2], gsh[n + u + 2], v2);
-                    v3 = fmaf(f[u + 3], gsh[n + u + 3], v3);
+                    v0 = fma((double)f[u + 0], gsh[n + u + 0], v0);
+                    v1 = fma((double)f[u + 1], gsh[n + u + 1], v1);
+                    v2 = fma((double)f[u + 2], gsh[n + u + 2], v2);
+                    v3 = fma((double)f[u + 3], gsh[n + u + 3], v3);
                 }
             }
             if (i < np) q[i] = ((v0 + v1) + (v2 + v3)) - gbg;
@@ -132,44 +137,35 @@ __global__ __launch_bounds__(256) void comp_bwd_kernel(const CompBwdParams cp) {
         for (int i = lane; i < np; i += 64) {
             const float sr = cp.sigma_raw[row0 + i];
             const float sg = fmaxf(sr, 0.0f);
-            const float e = expf(-sg * cp.delta[row0 + i]);
-            xx[i] = ((1.0f - (1.0f - e))) + 1e-10f;      // x = 1 - alpha + 1e-10 with alpha = 1 - e
+            xx[i] = exp(-(double)sg * cp.delta[row0 + i]) + 1e-10;      // x = 1 - alpha + 1e-10 with alpha = 1 - e
         }
     }
     __syncthreads();
     if (live && lane == 0) {
-        float T = 1.0f;
-        for (int i = 0; i < np; ++i) { TT[i] = T; T *= xx[i]; }
+        double T = 1.0;
+        for (int i = 0; i < np; ++i) { TT[i] = T; T = T * xx[i] < CB_LEAST ? 0.0 : T * xx[i]; }
     }
     __syncthreads();
     if (live) {
-        for (int i = lane; i < np; i += 64) {
-            const float sr = cp.sigma_raw[row0 + i];
-            const float e = expf(-fmaxf(sr, 0.0f) * cp.delta[row0 + i]);
-            const float alpha = 1.0f - e;
-            SS[i] = q[i] * alpha * TT[i];                 // q_i w_i
-        }
+        for (int i = lane; i < np; i += 64) SS[i] = q[i] * (1.0 + 1e-10 - xx[i]) * TT[i];       // q_i w_i
     }
     __syncthreads();
     if (live && lane == 0) {
-        float S = 0.0f;
-        for (int i = np - 1; i >= 0; --i) { const float t = SS[i]; SS[i] = S; S += t; }
+        double S = 0.0;
+        for (int i = np - 1; i >= 0; --i) { const double t = SS[i]; SS[i] = S; S += t; }
     }
     __syncthreads();
-    float cs = 0.0f, dsum = 0.0f;
+    double cs = 0.0, dsum = 0.0;
     if (live) {
         for (int i = lane; i < np; i += 64) {
             const float sr = cp.sigma_raw[row0 + i];
-            const float sg = fmaxf(sr, 0.0f);
-            const float dl = cp.delta[row0 + i];
-            const float e = expf(-sg * dl);
-            const float alpha = 1.0f - e;
-            const float dalpha = q[i] * TT[i] - SS[i] / xx[i];
-            cp.wglob[row0 + i] = alpha * TT[i];
-            const float dsr = sr > 0.0f ? dalpha * dl * e : 0.0f;
-            cp.dsig[row0 + i] = dsr;
+            const double sg = fmaxf(sr, 0.0f), dl = cp.delta[row0 + i], e = exp(-sg * dl);
+            const double dalpha = TT[i] * e < CB_LEAST ? 0.0 : q[i] * TT[i] - SS[i] / xx[i];
+            cp.wglob[row0 + i] = (float)((1.0 - e) * TT[i]);
+            const double dsr = sr > 0.0f ? dalpha * dl * e : 0.0;
+            cp.dsig[row0 + i] = (float)dsr;
             dsum += dsr;
-            cs = fmaf(dalpha * sg * e, dl, cs);
+            cs = fma(dalpha * sg * e, dl, cs);
         }
         // padded tail rows (i >= np) carry no gradient
         for (int i = np + lane; i < cpr * CHUNK; i += 64) { cp.wglob[row0 + i] = 0.0f; cp.dsig[row0 + i] = 0.0f; }
@@ -187,8 +183,8 @@ __global__ __launch_bounds__(256) void comp_bwd_kernel(const CompBwdParams cp) {
     dsum += __shfl_xor(dsum, 2);
     dsum += __shfl_xor(dsum, 1);
     if (live && lane == 0) {
-        cp.csum[ray] = cp.accumulate ? cp.csum[ray] + cs : cs;
-        cp.dsig_ray[ray] = dsum;
+        cp.csum[ray] = (float)(cp.accumulate ? cp.csum[ray] + cs : cs);
+        cp.dsig_ray[ray] = (float)dsum;
     }
 }
 
@@ -532,7 +528,7 @@ int run_bwd(const GnrProblem* p, int n_streams, const GnrWeights* const* w, cons
         cb.act_feat = ws.act_feat; cb.sigma_raw = ws.sigma_raw; cb.delta = fp.delta;
         cb.wglob = sc.wglob; cb.dsig = sc.dsig; cb.csum = sc.csum; cb.dsig_ray = sc.dsig_ray; cb.accumulate = s > 0;
         if (s == 0) stage_mark(GNR_STAGE_COMP_BWD, 0, st);
-        hipLaunchKernelGGL(comp_bwd_kernel, dim3((unsigned)((n_rays_total + 3) / 4)), dim3(256), 0, st, cb);
+        hipLaunchKernelGGL(comp_bwd_kernel, dim3((unsigned)((n_rays_total + 3) / 4)), dim3(256), cb_lds(p->n_samples), st, cb);
         if (s == 0) stage_mark(GNR_STAGE_COMP_BWD, 1, st);
         // 3. transposed weight stream
         PackTParams pt{};

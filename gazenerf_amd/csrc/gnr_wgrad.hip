@@ -1429,9 +1429,9 @@ void launch_wgrad_img(const float* A, int lda, int n_valid, const float* B, int 
 // per-image sum of a per-sample vector: out[b * out_stride] = sum_{s in image b} v[s]   (density bias gradient); one workgroup per
 // image, fixed order (round 5: one launch for all images; until then one launch per image)
 __global__ __launch_bounds__(256) void vecsum_kernel(const float* __restrict__ v, long per_image, float* __restrict__ out, int out_stride) {
-    __shared__ float red[256];
+    __shared__ double red[256];                   // 64 bits: the terms of a saturated density head nearly cancel
     const int b = blockIdx.x, tid = threadIdx.x;
-    float acc = 0.0f;
+    double acc = 0.0;
     for (long i = tid; i < per_image; i += 256) acc += v[(long)b * per_image + i];
     red[tid] = acc;
     __syncthreads();
@@ -1439,7 +1439,7 @@ __global__ __launch_bounds__(256) void vecsum_kernel(const float* __restrict__ v
         if (tid < s) red[tid] += red[tid + s];
         __syncthreads();
     }
-    if (tid == 0) out[(long)b * out_stride] = red[0];
+    if (tid == 0) out[(long)b * out_stride] = (float)red[0];
 }
 
 void launch_vecsum(const float* v, int batch, long per_image, float* out, int out_stride, hipStream_t stream) {
