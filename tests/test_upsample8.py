@@ -119,6 +119,61 @@ def test_image_from_a_map(feat_nc, n_blocks, min_feat, S, B, final):
     check(img, q, s, params, S, n_blocks, min_feat, final)
 
 
+def plain_network(x, params, n_blocks, min_feat, half):
+    """The network on x [B, C, S, S] in 64 bits -> the image before the sigmoid.  ``half`` > 0: where the definition rounds rows or weights to 8
+    bits, an error of its own, uniform in +- half a step, for every value."""
+    B, Cn, S, _ = x.shape
+    g = gen(17)
+
+    def row(t):
+        return t + (torch.rand(t.shape, generator=g, dtype=torch.float64) * 2 - 1) * half * (t.abs().amax(-1, keepdim=True) / 127) if half else t
+
+    def conv(t, name):
+        w = params[name + ".weight"].detach().cpu().double().reshape(-1, t.shape[-1])
+        y = t @ row(w).t() + params[name + ".bias"].detach().cpu().double()
+        return torch.maximum(y, 0.2 * y)
+
+    def rgb_conv(t, level):
+        w = params["feat_2_rgb_list.%d.weight" % level].detach().cpu().double().reshape(3, -1)
+        y = t @ w.t() + params["feat_2_rgb_list.%d.bias" % level].detach().cpu().double()
+        return y.transpose(1, 2).reshape(B, 3, S, S)
+
+    net = row(x.cpu().double().flatten(2).transpose(1, 2))
+    res, rgb = net, up_image(rgb_conv(net, 0))
+    for i in range(n_blocks):
+        c = net.shape[-1]
+        a2 = conv(row(conv(net, "feat_upsample_list.%d.layer_1" % i)), "feat_upsample_list.%d.layer_2" % i)
+        u = a2 + res[..., torch.arange(4 * c) % c]
+        u = u.reshape(B, S, S, c, 2, 2).permute(0, 3, 1, 4, 2, 5).reshape(B * c, 1, 2 * S, 2 * S)
+        k = torch.tensor([0.25, 0.5, 0.25], dtype=torch.float64)
+        v = F.conv2d(F.pad(u, (1, 1, 1, 1), mode="reflect"), (k[:, None] * k[None, :])[None, None])
+        S *= 2
+        net = conv(row(v.reshape(B, c, S * S).transpose(1, 2)), "feat_layers.%d" % i)
+        rgb, res = rgb + rgb_conv(net, i + 1), net
+        if i < n_blocks - 1:
+            rgb, net = up_image(rgb), row(net)
+    return rgb
+
+
+@gpu
+@pytest.mark.parametrize("feat_nc, n_blocks, min_feat, B", [(36, 2, 8, 2), (258, 3, 32, 1)])
+def test_the_8_bit_image_is_as_near_to_the_fp32_one_as_rounding_says(feat_nc, n_blocks, min_feat, B):
+    """What 8 bits cost: the rms difference to the fp32 renderer's image against that of the network in 64 bits with an independent error, uniform
+    in +- half a step, at every 8-bit rounding.  Rounding errors are as large as that and nearly independent; two of them that were not would
+    add up to at most twice the rms.  (bf16 between the products adds 2^-9 of a value where 8 bits add 2^-8 of the row's largest: inside.)"""
+    params = make_params(feat_nc, n_blocks, min_feat, feat_nc + 1)
+    x = features((B, feat_nc, 16, 16), 1, feat_nc).to(DEV)
+    rms = lambda t: float(t.double().pow(2).mean().sqrt())
+    with torch.no_grad():
+        exact = G.neural_render(x, params, n_blocks, min_feat, False).cpu().double()
+        d = rms(G.neural_render_int8(x, params, n_blocks, min_feat, False).cpu().double() - exact)
+    plain = plain_network(x, params, n_blocks, min_feat, 0.0)
+    model = rms(plain_network(x, params, n_blocks, min_feat, 1.0 / 2) - plain)
+    print("8-bit rms error %.3e, of independent roundings %.3e, image rms %.3e" % (d, model, rms(exact)))
+    assert rms(exact - plain) < 1e-4 * rms(plain)                    # the same network
+    assert d <= 2 * model and model < 0.1 * rms(plain)
+
+
 @gpu
 def test_image_from_cached_rows():
     """The same bits from the slots of a cache; padding slots are zero maps, slots outside the cache NaN images."""
