@@ -26,6 +26,7 @@ import operator
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, _torch_ext
 from .render import _ext_call, _has_tangent, _stream_ptr
@@ -71,9 +72,10 @@ def _one_device(**ts):
 
 
 def _no_grad(what, *ts):
-    if torch._C._is_tracing():                      # torch.jit.is_tracing() at a third of its time: a call of one row takes 5 us
+    # a call of one row takes 5 us: torch.jit.is_tracing() at a third of its time, and no look at the tensors while no dual level is open
+    if torch._C._is_tracing():
         raise RuntimeError("%s cannot be traced: the trace would hold its result as a constant" % what)
-    if _has_tangent(*ts):
+    if forward_ad._current_level >= 0 and _has_tangent(*ts):
         raise RuntimeError("%s has no forward-mode gradient: call it on inputs without a tangent (torch.autograd.forward_ad)" % what)
     if torch.is_grad_enabled():
         for t in ts:
