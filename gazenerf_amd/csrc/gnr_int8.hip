@@ -48,26 +48,22 @@ __device__ __forceinline__ float x_scale(const Int8Args& a, long b, long r, bool
 __device__ __forceinline__ float leak(float v) { return fmaxf(v, 0.2f * v); }
 
 // sum * x_scale * w_scale + bias in this order, two roundings; the same order for both layouts, hence the same bits.  The first product can
-// leave fp32's normal range where the result does not: |sum| <= 2^31, so only for an x_scale `far` from 1 (a row whose largest value exceeds
-// 2^103, a subnormal scale).  Then 2^64 goes from one scale to the other, exactly for every result in range.  FAR is one answer for a wave or
-// a workgroup and chooses between two epilogues: a test of every product cost 28672 x 516 -> 1032 2.4 us of 46.4, a branch for four of them 1.5.
+// leave fp32's normal range where the result does not: |sum| <= 2^31, so only for an x_scale FAR from 1 (a row whose largest value exceeds
+// 2^103, a subnormal scale).  Then 2^64 goes from one scale to the other, exactly for every result in range.  A wave that sees no such scale
+// does without: a test of every product cost 28672 x 516 -> 1032 2.4 us of 46.4.
 __device__ __forceinline__ bool scale_is_far(float s) {
     const float m = fabsf(s);
     return m > 0x1p96f || (m < 0x1p-126f && m > 0.0f);
 }
-template <bool FAR> __device__ __forceinline__ fv4 scaled(fv4 sum, fv4 sx, fv4 sw, fv4 b) {
-    constexpr int INF = 0x204, SUBNORMAL = 0x090;              // of v_cmp_class, both signs
-    fv4 v;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = fmaf(sum[r] * sx[r], sw[r], b[r]);
-    if constexpr (FAR)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float t = sum[r] * sx[r];
-            if (__builtin_amdgcn_classf(t, INF)) v[r] = fmaf(sum[r] * (sx[r] * 0x1p-64f), sw[r] * 0x1p64f, b[r]);
-            else if (__builtin_amdgcn_classf(t, SUBNORMAL)) v[r] = fmaf(sum[r] * (sx[r] * 0x1p64f), sw[r] * 0x1p-64f, b[r]);
-        }
-    return v;
+template <bool FAR> __device__ __forceinline__ float scaled(float sum, float sx, float sw, float b) {
+    if constexpr (FAR) {
+        constexpr int INF = 0x204, SUBNORMAL = 0x090;          // of v_cmp_class, both signs
+        const float t = sum * sx;
+        const bool big = __builtin_amdgcn_classf(t, INF), small = __builtin_amdgcn_classf(t, SUBNORMAL);
+        sx *= big ? 0x1p-64f : (small ? 0x1p64f : 1.0f);
+        sw *= big ? 0x1p64f : (small ? 0x1p-64f : 1.0f);
+    }
+    return fmaf(sum * sx, sw, b);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -121,7 +117,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void int8_tile_kernel(const Int8Ar
     constexpr int EM = 32 * PAIR, RB = EM * (int)sizeof(T), PPR = RB / 16;     // their row of m: values, bytes, 16-byte pieces
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     __shared__ __attribute__((aligned(16))) float sc[ROWS], bi[CF ? BN : BM];
-    __shared__ int far_s;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
     const int half = lane >> 5, sw = (lane >> 1) & 3, piece = (lane & 3) ^ ((lane >> 3) & 3);
     const long M = CF ? a.P : a.O, N = CF ? a.O : a.N;
@@ -141,7 +136,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void int8_tile_kernel(const Int8Ar
     }
     constexpr int SCN = (ROWS + NT - 1) / NT;
     float rs[SCN], rz[SCN];                                    // scales and bias of the tile's rows: requested first, needed last
-    if (tid == 0) far_s = 0;                                   // barriers until the scales are stored
 #pragma unroll
     for (int j = 0; j < SCN; ++j) {
         const int i = tid + j * NT;
@@ -226,7 +220,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void int8_tile_kernel(const Int8Ar
         const int i = tid + j * NT;
         if (i < ROWS) {
             sc[i] = rs[j];
-            if ((i < BM) == CF && scale_is_far(rs[j])) far_s = 1;
             if ((i < BM) != CF) bi[i < BM ? i : i - BM] = rz[j];
         }
     }
@@ -238,51 +231,72 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void int8_tile_kernel(const Int8Ar
     // fp32 26764 x 624 -> 4092 232 / 184, maps of 233 x 220001 -> 570 362 / 195)
     const bool inside = m0 + BM <= M && n0 + BN <= N, past = M * sizeof(T) % 128 == 0 || (!CF && sizeof(T) == 2 && a.N * a.O * (long)sizeof(T) >= CACHES);
     const int mw = 32 * TM * wm;
-    auto epilogue = [&](auto is_far) {
+    // a scale far from 1 among the wave's rows: value by value through LDS in a loop, stored as they come.  (Unrolled, or as a second copy of
+    // the epilogue below, it takes 57 registers more: two waves a SIMD instead of four, 28672 x 258 -> 516 25 us instead of 21.)
+    const float* xsc = CF ? sc + mw : sc + BM + 32 * TN * wn;
+    bool far = false;
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const int nl = 32 * (wn * TN + j), nr = lane & 31;
-            const float sn = sc[BM + nl + nr], bn = CF ? bi[nl + nr] : 0.0f;
-            T* yn = (T*)a.y + b * (long)a.O * a.P + (n0 + nl) * M + m0 + mw;
+    for (int i = 0; i < (CF ? TM : TN); ++i) far |= scale_is_far(xsc[32 * i + (lane & 31)]);
+    if (__any(far)) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int ml = 8 * q + 4 * half;
-                    const fv4 sm = *(const fv4*)(sc + mw + 32 * i + ml), bm = CF ? fv4{bn, bn, bn, bn} : *(const fv4*)(bi + mw + 32 * i + ml);
-                    typedef T t4 __attribute__((ext_vector_type(4)));
-                    t4 o;
-                    fv4 sum;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) sum[r] = (float)acc[i][j][4 * q + r];
-                    const fv4 s4 = fv4{sn, sn, sn, sn}, v = scaled<decltype(is_far)::value>(sum, CF ? sm : s4, CF ? s4 : sm, bm);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) o[r] = (T)(a.leaky ? leak(v[r]) : v[r]);
-                    const int at = 32 * (i % PAIR) + ml;
-                    if constexpr (sizeof(T) == 4) *(t4*)(turn + nr * RB + 16 * ((at >> 2) ^ (nr & (PPR - 1)))) = o;
-                    else *(t4*)(turn + nr * RB + 16 * ((at >> 3) ^ (nr & (PPR - 1))) + 2 * (at & 4)) = o;
+                for (int q = 0; q < 4; ++q) *(i32x4*)(turn + 1024 * q + 16 * lane) = i32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+#pragma unroll 1
+                for (int r = 0; r < 16; ++r) {
+                    const int ml = mw + 32 * i + 8 * (r >> 2) + 4 * half + (r & 3), nl = 32 * (wn * TN + j) + (lane & 31);
+                    if (m0 + ml < M && n0 + nl < N) {
+                        float v = scaled<true>((float)*(const int*)(turn + 1024 * (r >> 2) + 16 * lane + 4 * (r & 3)), sc[CF ? ml : BM + nl], sc[CF ? BM + nl : ml], bi[CF ? nl : ml]);
+                        if (a.leaky) v = leak(v);
+                        ((T*)a.y)[b * (long)a.O * a.P + (n0 + nl) * M + m0 + ml] = (T)v;
+                    }
                 }
-                if (i % PAIR == PAIR - 1) {
+            }
+        return;
+    }
 #pragma unroll
-                    for (int it = 0; it < 32 * PPR / 64; ++it) {
-                        const int row = it * (64 / PPR) + lane / PPR, pc = lane % PPR;
-                        Vec<T> o;
-                        __builtin_memcpy(&o, __builtin_assume_aligned(turn + row * RB + 16 * (pc ^ (row & (PPR - 1))), 16), 16);
-                        const int ml = 32 * (i - PAIR + 1) + Vec<T>::N * pc;
-                        T* p = yn + row * M + ml;
-                        if (inside && past) store_part<true>(p, o, Vec<T>::N);
-                        else if (inside) store_part(p, o, Vec<T>::N);
-                        else if (n0 + nl + row < N && m0 + mw + ml < M) {
-                            const long left = M - m0 - mw - ml;
-                            store_part(p, o, left < Vec<T>::N ? (int)left : Vec<T>::N);
-                        }
+    for (int j = 0; j < TN; ++j) {
+        const int nl = 32 * (wn * TN + j), nr = lane & 31;
+        const float sn = sc[BM + nl + nr], bn = CF ? bi[nl + nr] : 0.0f;
+        T* yn = (T*)a.y + b * (long)a.O * a.P + (n0 + nl) * M + m0 + mw;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int ml = 8 * q + 4 * half;
+                const fv4 sm = *(const fv4*)(sc + mw + 32 * i + ml), bm = CF ? fv4{bn, bn, bn, bn} : *(const fv4*)(bi + mw + 32 * i + ml);
+                typedef T t4 __attribute__((ext_vector_type(4)));
+                t4 o;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float v = scaled<false>((float)acc[i][j][4 * q + r], CF ? sm[r] : sn, CF ? sn : sm[r], bm[r]);
+                    if (a.leaky) v = leak(v);
+                    o[r] = (T)v;
+                }
+                const int at = 32 * (i % PAIR) + ml;
+                if constexpr (sizeof(T) == 4) *(t4*)(turn + nr * RB + 16 * ((at >> 2) ^ (nr & (PPR - 1)))) = o;
+                else *(t4*)(turn + nr * RB + 16 * ((at >> 3) ^ (nr & (PPR - 1))) + 2 * (at & 4)) = o;
+            }
+            if (i % PAIR == PAIR - 1) {
+#pragma unroll
+                for (int it = 0; it < 32 * PPR / 64; ++it) {
+                    const int row = it * (64 / PPR) + lane / PPR, pc = lane % PPR;
+                    Vec<T> o;
+                    __builtin_memcpy(&o, __builtin_assume_aligned(turn + row * RB + 16 * (pc ^ (row & (PPR - 1))), 16), 16);
+                    const int ml = 32 * (i - PAIR + 1) + Vec<T>::N * pc;
+                    T* p = yn + row * M + ml;
+                    if (inside && past) store_part<true>(p, o, Vec<T>::N);
+                    else if (inside) store_part(p, o, Vec<T>::N);
+                    else if (n0 + nl + row < N && m0 + mw + ml < M) {
+                        const long left = M - m0 - mw - ml;
+                        store_part(p, o, left < Vec<T>::N ? (int)left : Vec<T>::N);
                     }
                 }
             }
         }
-    };
-    if (__builtin_amdgcn_readfirstlane(far_s)) epilogue(std::true_type{});
-    else epilogue(std::false_type{});
+    }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -416,19 +430,16 @@ __global__ __launch_bounds__(256) void int8_few_kernel(const Int8Args a) {
         const float sx = xsc[n];
         const unsigned P = (unsigned)a.P, at = (unsigned)(n0 + n);
         T* y = CF ? (T*)a.y + (long)(at / P) * a.O * P + at % P : (T*)a.y + (n0 + n) * a.O;
-        fv4 sw, sb, sf;
+        const bool far = __any(scale_is_far(sx));
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int oo = o0 + 4 * (lane >> 4) + r;
-            sw[r] = oo < a.O ? a.ws[oo] : 0.0f;
-            sb[r] = oo < a.O && a.bias ? a.bias[oo] : 0.0f;
-            sf[r] = (float)sum[r];
-        }
-        const fv4 sx4 = {sx, sx, sx, sx}, v = __any(scale_is_far(sx)) ? scaled<true>(sf, sx4, sw, sb) : scaled<false>(sf, sx4, sw, sb);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int oo = o0 + 4 * (lane >> 4) + r;
-            if (oo < a.O) y[CF ? (long)oo * P : (long)oo] = (T)(a.leaky ? leak(v[r]) : v[r]);
+            if (oo < a.O) {
+                const float wb = a.bias ? a.bias[oo] : 0.0f;
+                float v = far ? scaled<true>((float)sum[r], sx, a.ws[oo], wb) : scaled<false>((float)sum[r], sx, a.ws[oo], wb);
+                if (a.leaky) v = leak(v);
+                y[CF ? (long)oo * P : (long)oo] = (T)v;
+            }
         }
     }
 }
@@ -591,13 +602,11 @@ __global__ __launch_bounds__(256) void int8_fused_kernel(const Int8Args a, unsig
                         bm[r] = __shfl(wb, ml + r);
                     }
                 }
-                fv4 sum;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sum[r] = (float)acc[4 * q + r];
-                v = scaled<decltype(is_far)::value>(sum, CF ? sm : fv4{xn, xn, xn, xn}, CF ? fv4{wsc, wsc, wsc, wsc} : sm, bm);
-                if (a.leaky)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] = leak(v[r]);
+                for (int r = 0; r < 4; ++r) {
+                    v[r] = scaled<decltype(is_far)::value>((float)acc[4 * q + r], CF ? sm[r] : xn, CF ? wsc : sm[r], bm[r]);
+                    if (a.leaky) v[r] = leak(v[r]);
+                }
                 *(fv4*)(turn + nr * 32 + 4 * ((ml >> 2) ^ (nr & 7))) = v;
             }
         };
