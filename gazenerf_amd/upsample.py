@@ -201,6 +201,8 @@ class RecentlyUsed:
 
     def room(self) -> bool:
         """May ``put`` be called for a new key?  Makes room where it may."""
+        if self.most < 1:
+            return False
         if len(self.values) >= self.most:
             oldest = min(self.used, key=self.used.get)
             if self.lookups - self.used[oldest] <= 8 * self.most:

@@ -325,6 +325,7 @@ def test_more_streams_than_renderers(monkeypatch):
         assert [on(h) for h in range(5)] == first
     assert [on(4) for _ in range(40)][-1] is not None and len(renderers.streams) == 4     # the other four fell silent
     assert sum(on(h) is None for h in range(5)) == 1
+    assert upsample8.Int8Renderers(0)(dev) is None                                        # none kept: every call without a graph
 
 
 @gpu
