@@ -41,7 +41,7 @@ template <typename T> __device__ __forceinline__ Vec<T> load_part(const T* p, in
     return r;
 }
 constexpr long CACHES = 256L << 20;                      // bytes behind the L2s
-// STREAM: a result that exceeds the caches goes past them (gnr_quant.hip, read_maps_kernel: 112 -> 51 us)
+// STREAM: a result that exceeds the caches goes past them (gnr_quant.hip, read_maps_kernel on rows that the caches hold: 112 -> 51 us)
 template <bool STREAM = false, typename T> __device__ __forceinline__ void store_part(T* p, const Vec<T>& r, int n) {
     if (n >= Vec<T>::N) {
         if constexpr (STREAM) {

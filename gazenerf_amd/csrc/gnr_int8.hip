@@ -731,9 +731,9 @@ template <typename X, typename T, bool CF, int TT> static void launch_few(const 
 //   little of y           the same with blocks of 16 or 32 rows, while a CU has about one: what counts is how K is shared (150 x 1422 -> 256: 4.0 /
 //                         6.5, 100 x 2048 -> 834: 6.3 / 8.0; 512 x 2048 -> 834, 848 blocks of 32: 14.8 / 8.2)
 //   O <= 32, 64           tiles as narrow as the layer (262144 x 64 -> 32, fp32 maps: 8.0 against 9.0 with 64 rows a wave)
-//   256 x 256 tiles       where K is long, they fill the card and few of their values fall outside: 16384 x 2048 -> 4096 150 / 221
-//                         with 128 x 128, but 28672 x 516 -> 1032 (a fifth outside) 43 / 41 and 28672 x 258 -> 516 23 / 18
-//   128 x 256 rows        for K as long otherwise: 28672 x 516 -> 1032 36 / 41; with few of them 8192 x 516 -> 1032 15.8 / 15.0
+//   256 x 256 tiles       where K is long, they fill the card and few of their values fall outside: 16384 x 2048 -> 4096 144 / 202
+//                         with 128 x 128 (the products alone; 141 / 188 at best), but 28672 x 516 -> 1032 (a fifth outside) 43 / 41 and 28672 x 258 -> 516 23 / 18
+//   128 x 256 rows        for K as long otherwise: 28672 x 516 -> 1032 39 / 43; with few of them 8192 x 516 -> 1032 15.8 / 15.0
 //   128 x 128, 64 x 64    by whether the larger fill the card (4096 x 258 -> 516, fp32: 64 x 64 6.2, 128 x 128 8.3)
 template <typename T, bool CF> static int launch_int8(const Int8Args& a, long batch, hipStream_t st) {
     const long few = (a.N + 15) / 16 * ((a.O + 15) / 16), few2 = (a.N + 31) / 32 * ((a.O + 15) / 16);

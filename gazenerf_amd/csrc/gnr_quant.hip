@@ -3,7 +3,8 @@
 // Mathematics: gnr_int8.h.  All three kernels are bound by memory: a value is read once (4 or 2 bytes) and written once (1 byte),
 // or the other way round, with some ten operations in between.  What they are built around is the change of layout: maps are
 // channels first (a channel's pixels contiguous), rows are pixels first (a pixel's channels contiguous), so a workgroup owns a
-// tile of pixels whose 128 bytes per channel are whole lines, and the bytes change sides in LDS.
+// tile of pixels -- 32 of them: 128 bytes of a channel in fp32, a whole line, 64 in 16 bits; half of that while there are few tiles -- and the
+// bytes change sides in LDS.
 #include "gnr_int8.h"
 
 namespace gnr {
@@ -17,7 +18,8 @@ __device__ __forceinline__ long tile_start(unsigned i, int tp, long n) {
 // channels-first maps [B][C][P] -> rows.  A tile is 32 pixels: LPX lanes x 16 bytes cover them in one channel (a line of 128 bytes in
 // fp32), a thread keeps R quads of channels in registers between the row maximum and the quantisation, so x is read once up to
 // 2048 channels (fp32; 4096 in 16 bits: 1024 threads, R = 4); wider rows are read twice.  Bound by memory: 64 maps of 258 x 4096 in
-// fp32 (339 MB) take 78 us = 4.3 TB/s, 16 maps of 1024 x 4096 in fp16 (202 MB) 44 us = 4.6 TB/s; a large copy on this card: 4.7.
+// fp32 (339 MB) take 87 us = 3.9 TB/s, 32 of them (170 MB) 52 us = 3.3, 8 maps of 1024 x 4096 in fp16 (101 MB, half lines) 34 us = 3.0; a large
+// copy on this card: 4.7.
 // ---------------------------------------------------------------------------------------------
 template <typename T, int LPX, int R>
 __global__ __launch_bounds__(1024) void quant_maps_kernel(const GnrRowsProblem p, unsigned tiles, int ld) {
@@ -186,7 +188,8 @@ template <typename T> __device__ __forceinline__ T row_value(int q, float s) {
 // cached rows -> channels-first maps [B][C][P].  A tile's rows go to LDS whole and ONE barrier later the workgroup only stores: with a
 // barrier per 128 channels every one of them waited for the stores before it.  The stores bypass the caches: four bytes leave for each
 // that came, and through the caches they push out the rows that the neighbouring tile is about to read.  64 maps of 258 x 4096, fp32
-// (339 MB): 112 us through the caches, 51 us = 6.6 TB/s past them.  (The tile -> XCD order of quant_maps_kernel costs here: 54 us.)
+// (339 MB), the same again and again, so that their rows (72 MB) stay in the caches: 112 us with stores through them, 51 us past them (in the
+// tile -> XCD order of quant_maps_kernel 54).  Rows that come from memory: 73 us = 4.6 TB/s.
 // ---------------------------------------------------------------------------------------------
 template <typename T, int LPX>
 __global__ __launch_bounds__(256) void read_maps_kernel(const GnrRowsProblem p, unsigned tiles, unsigned parts, int ld, int step) {
