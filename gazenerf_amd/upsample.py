@@ -10,6 +10,7 @@ CUDA (ROCm) float32 tensors only; no CPU fallback.
 from __future__ import annotations
 
 import ctypes as C
+import gc
 import math
 import threading
 from typing import Dict
@@ -175,9 +176,14 @@ def capture_graph(dev, call):
         with torch.cuda.stream(stream):
             call()
         current.wait_stream(stream)
-        graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
-            call()
+        graph, collecting = torch.cuda.CUDAGraph(), gc.isenabled()
+        gc.disable()                       # the end of a dead graph waits for the device, and during a capture that ends the process
+        try:
+            with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+                call()
+        finally:
+            if collecting:
+                gc.enable()
     return graph
 
 

@@ -6,6 +6,8 @@ GPU: the HIP kernels behind gnr_upsample_fwd / gnr_upsample_bwd against the same
 Tolerances: image 1e-4 max-abs (applied to the sigmoid image); gradients rel-L2 1e-3
 (exact-fp32 MFMA GEMMs; only the summation order differs from the reference).
 """
+import gc
+
 import numpy as np
 import pytest
 import torch
@@ -489,8 +491,12 @@ def test_graphs_are_captured_on_a_stream_nobody_else_gets():
     meanwhile: the capture stream is not among them, and captures use it alone."""
     from gazenerf_amd import upsample
     dev = _dev()
-    seen = []
-    upsample.capture_graph(dev, lambda: seen.append(torch.cuda.current_stream(dev).cuda_stream))
+    seen, collecting = [], []
+    upsample.capture_graph(dev, lambda: (seen.append(torch.cuda.current_stream(dev).cuda_stream), collecting.append(gc.isenabled())))
+    assert collecting == [True, False] and gc.isenabled()            # a collection during a capture could end a dead graph, which waits for the device
+    with pytest.raises(ZeroDivisionError):
+        upsample.capture_graph(dev, lambda: 1 / 0)
+    assert gc.isenabled() and not upsample._CAPTURE.locked()
     own = upsample._CAPTURE_STREAMS[dev.index or 0].cuda_stream
     assert seen == [own, own]
     assert own not in {torch.cuda.Stream().cuda_stream for _ in range(200)} | {torch.cuda.default_stream().cuda_stream}
