@@ -82,13 +82,15 @@ struct CompBwdParams {
     int accumulate;
 };
 
-// Accumulated in 64 bits: q_i and the weighted mean of the q_j behind it nearly cancel where the density head saturates, and a sum of the
-// terms' gradients cancels once more (density bias: |sum| down to 1/36 of the sum of magnitudes).  In fp32 the rounding of q, of the suffix sums
-// and of S / x was 3-10 x the rest of the pass's error there.  The kernel waits for memory: same time.  What less than CB_LEAST of a ray's light
-// reaches (1e-24; in fp32 the products below 1e-38 vanished) counts as 0: it would only leave gradients under fp32's normal range behind,
-// which are not linear in the upstream gradient any more.
+// What nearly cancels is held in 64 bits: where the density head saturates, q_i against the mean of the q_j behind it,
+//   dL/da_i = T_i (q_i - R_i),   R_{i-1} = a_i q_i + x_i R_i,   R_last = 0
+// (R_i = sum_{j>i} q_j w_j / T_{i+1}; the difference is taken before T_i comes in), and then the terms' sum (density bias: |sum| down to 1/36 of the
+// sum of magnitudes).  In fp32 the rounding of q, of suffix sums and of their quotient by x left 3-10 x the rest of the pass's error there.
+// T_i and e_i only scale a difference: fp32, so that the LDS of a ray is the 16 bytes a sample that it was, and four workgroups fit a CU at 512.
+// What less than CB_LEAST of a ray's light reaches (1e-24; in fp32 the products below 1e-38 vanished) counts as 0: it would only leave
+// gradients under fp32's normal range behind, which are not linear in the upstream gradient any more.
 constexpr double CB_LEAST = 0x1p-80;
-constexpr size_t cb_lds(int np) { return sizeof(double) * (4 * 4 * (size_t)np + 4 * FEAT_PAD); }       // q, x, T, S and g of four rays
+constexpr size_t cb_lds(int np) { return 4 * (sizeof(double) * (size_t)np + sizeof(float) * (2 * (size_t)np + FEAT_PAD)); }      // q, e, T and g of four rays
 
 __global__ __launch_bounds__(256) void comp_bwd_kernel(const CompBwdParams cp) {
     extern __shared__ double cb_smem[];
@@ -98,7 +100,8 @@ __global__ __launch_bounds__(256) void comp_bwd_kernel(const CompBwdParams cp) {
     const long ray = (long)blockIdx.x * 4 + wave;
     const bool live = ray < n_rays_total;
     const int np = p.n_samples, cpr = cp.chunks_per_ray;
-    double *q = cb_smem + wave * (4 * np + FEAT_PAD), *xx = q + np, *TT = xx + np, *SS = TT + np, *gsh = SS + np;
+    double* q = cb_smem + wave * np;
+    float *ee = (float*)(cb_smem + 4 * np) + wave * (2 * np + FEAT_PAD), *TT = ee + np, *gsh = TT + np;
     const long row0 = live ? ray * cpr * CHUNK : 0;       // padded rows of this ray are contiguous
 
     // q_i = g . feat_i - g_bg: the features are CCM ([chunk][288][32]), so a lane owns one sample and
@@ -123,45 +126,60 @@ __global__ __launch_bounds__(256) void comp_bwd_kernel(const CompBwdParams cp) {
                 for (int u = 0; u < 16; ++u) f[u] = __builtin_nontemporal_load(fr + (n + u) * CHUNK);
 #pragma unroll
                 for (int u = 0; u < 16; u += 4) {
-                    v0 = fma((double)f[u + 0], gsh[n + u + 0], v0);
-                    v1 = fma((double)f[u + 1], gsh[n + u + 1], v1);
-                    v2 = fma((double)f[u + 2], gsh[n + u + 2], v2);
-                    v3 = fma((double)f[u + 3], gsh[n + u + 3], v3);
+                    v0 = fma((double)f[u + 0], (double)gsh[n + u + 0], v0);
+                    v1 = fma((double)f[u + 1], (double)gsh[n + u + 1], v1);
+                    v2 = fma((double)f[u + 2], (double)gsh[n + u + 2], v2);
+                    v3 = fma((double)f[u + 3], (double)gsh[n + u + 3], v3);
                 }
             }
             if (i < np) q[i] = ((v0 + v1) + (v2 + v3)) - gbg;
         }
     }
     __syncthreads();
+    if (live)
+        for (int i = lane; i < np; i += 64) ee[i] = (float)exp(-(double)fmaxf(cp.sigma_raw[row0 + i], 0.0f) * cp.delta[row0 + i]);
+    __syncthreads();
     if (live) {
-        for (int i = lane; i < np; i += 64) {
-            const float sr = cp.sigma_raw[row0 + i];
-            const float sg = fmaxf(sr, 0.0f);
-            xx[i] = exp(-(double)sg * cp.delta[row0 + i]) + 1e-10;      // x = 1 - alpha + 1e-10 with alpha = 1 - e
+        // both recursions as scans over the lanes, each with a run of neighbouring samples (x = 1 - a + 1e-10 = e + 1e-10): T as a product, R as the
+        // composition of the maps R -> b + x R of the samples behind.  One lane walking all samples took 0.43 ms at 512 of them, 0.37 now.
+        const int run = (np + 63) >> 6, i0 = lane * run < np ? lane * run : np, i1 = i0 + run < np ? i0 + run : np;
+        double A = 1.0, B = 0.0;
+        for (int i = i1 - 1; i >= i0; --i) {
+            const double e = ee[i], x = e + 1e-10;
+            B = (1.0 - e) * q[i] + x * B;
+            A *= x;
         }
-    }
-    __syncthreads();
-    if (live && lane == 0) {
-        double T = 1.0;
-        for (int i = 0; i < np; ++i) { TT[i] = T; T = T * xx[i] < CB_LEAST ? 0.0 : T * xx[i]; }
-    }
-    __syncthreads();
-    if (live) {
-        for (int i = lane; i < np; i += 64) SS[i] = q[i] * (1.0 + 1e-10 - xx[i]) * TT[i];       // q_i w_i
-    }
-    __syncthreads();
-    if (live && lane == 0) {
-        double S = 0.0;
-        for (int i = np - 1; i >= 0; --i) { const double t = SS[i]; SS[i] = S; S += t; }
+        double P = A;                                         // inclusive product over the lanes in front
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const double p1 = __shfl_up(P, m), a1 = __shfl_down(A, m), b1 = __shfl_down(B, m);
+            if (lane >= m) P *= p1;
+            if (lane + m < 64) {                              // inclusive composition with the lanes behind
+                B += A * b1;
+                A *= a1;
+            }
+        }
+        double T = __shfl_up(P, 1), R = __shfl_down(B, 1);
+        T = lane ? T : 1.0;
+        R = lane < 63 ? R : 0.0;
+        for (int i = i0; i < i1; ++i) {
+            TT[i] = T < CB_LEAST ? 0.0f : (float)T;
+            T *= ee[i] + 1e-10;
+        }
+        for (int i = i1 - 1; i >= i0; --i) {
+            const double t = q[i], e = ee[i];
+            q[i] = t - R;
+            R = (1.0 - e) * t + (e + 1e-10) * R;
+        }
     }
     __syncthreads();
     double cs = 0.0, dsum = 0.0;
     if (live) {
         for (int i = lane; i < np; i += 64) {
             const float sr = cp.sigma_raw[row0 + i];
-            const double sg = fmaxf(sr, 0.0f), dl = cp.delta[row0 + i], e = exp(-sg * dl);
-            const double dalpha = TT[i] * e < CB_LEAST ? 0.0 : q[i] * TT[i] - SS[i] / xx[i];
-            cp.wglob[row0 + i] = (float)((1.0 - e) * TT[i]);
+            const double sg = fmaxf(sr, 0.0f), dl = cp.delta[row0 + i], e = exp(-sg * dl), T = TT[i];
+            const double dalpha = T * e < CB_LEAST ? 0.0 : q[i] * T;
+            cp.wglob[row0 + i] = (float)((1.0 - e) * T);
             const double dsr = sr > 0.0f ? dalpha * dl * e : 0.0;
             cp.dsig[row0 + i] = (float)dsr;
             dsum += dsr;
